@@ -44,7 +44,12 @@ enum musc_b200_status {
                                   musc_b200_take_device_error) */
 };
 
-enum musc_b200_dtype { MUSC_B200_F32 = 0, MUSC_B200_F16 = 1, MUSC_B200_BF16 = 2 };
+enum musc_b200_dtype {
+  MUSC_B200_F32 = 0,
+  MUSC_B200_F16 = 1,
+  MUSC_B200_BF16 = 2,
+  MUSC_B200_E4M3 = 3 /* 8 bits; an output of musc_b200_add_rmsnorm only */
+};
 
 /* ABI version of this header (bumped on any signature change): 3. */
 int musc_b200_abi_version(void);
@@ -372,6 +377,93 @@ int musc_b200_attention_fwd(const void* q, const void* k, const void* v, void* o
 int musc_b200_add_layernorm(float* x, const void* delta, int delta_dtype, const float* gamma,
                             const float* beta, float eps, void* out, int out_dtype, long long rows,
                             int channels, musc_b200_stream stream);
+
+/* Residual add + root-mean-square norm of a block that keeps no mean, beside
+ * musc_b200_add_layernorm.  Per row (rows x_stride, delta_stride, out_stride
+ * elements apart): h = x + delta in fp32 (delta NULL = no add), x = h rounded to
+ * x_dtype (untouched without delta), y = h / sqrt(mean(h^2) + eps) * weight from
+ * the unrounded h.  x and delta f32, f16 or bf16; weight [channels] f32.  out: y in
+ * f32, f16 or bf16, or e4m3: out = y / scale rounded to nearest, with
+ * scales [rows][ceil(channels / group)] fp32 = max |y| / 448 over the row (group
+ * 0: one scale) or over each group of 32, 64, 128 or 256 columns (a row or
+ * group of zeros: 2^-126).  1 <= channels <= 32768, any alignment (16-byte
+ * vectors are used where every row starts on 16 bytes and channels % 8 == 0);
+ * the memory ranges of x, delta, out and scales must not overlap.  rows == 0 does nothing. */
+int musc_b200_add_rmsnorm(void* x, int x_dtype, const void* delta, int delta_dtype, const float* weight,
+                          float eps, void* out, int out_dtype, float* scales, int group, long long rows,
+                          int channels, long long x_stride, long long delta_stride, long long out_stride,
+                          musc_b200_stream stream);
+
+/* Rotary positions over one or several axes (time, rows, columns), in the place
+ * of the learned positions that the vision tower adds to its tokens
+ * (models/backbone/open_clip/transformer.py:570-574) where grids differ in size.
+ * Pair p < pairs of every head turns by positions[token][axis[p]] * frequencies[p]:
+ *   y0 = x0 cos - x1 sin,  y1 = x1 cos + x0 sin,
+ * (x0, x1) = dims (p, p + pairs), or (2p, 2p + 1) with adjacent != 0; dims past
+ * 2 * pairs are copied.  q: [tokens][heads][head_dim], k: [tokens][kv_heads][head_dim]
+ * (kv_heads 0: no k), rows at the given strides (elements); f32, f16 or bf16,
+ * rotated in fp32 and rounded once; angles are formed in fp64.  positions:
+ * [tokens][axes] int32, or fp32 with float_positions != 0; axis[p] outside
+ * [0, axes) is clamped.  An output may be its own input (in place) and must not
+ * overlap anything else.  head_dim <= 512.  tokens == 0 does nothing. */
+int musc_b200_rotary(const void* q, const void* k, void* q_out, void* k_out, int dtype, long long tokens,
+                     int heads, int kv_heads, int head_dim, long long q_stride, long long k_stride,
+                     long long q_out_stride, long long k_out_stride, const void* positions,
+                     int float_positions, int axes, const float* frequencies, const int* axis, int pairs,
+                     int adjacent, musc_b200_stream stream);
+
+/* ------------------------------------------------------------------------
+ * Masked attention over documents, beside musc_b200_attention_fwd: rows of several
+ * images or texts packed into one sequence, padded batches, or new tokens
+ * against a cache of keys.  A query row i of a document with nq query rows and
+ * nk keys attends to that document's keys j:
+ *   z = scale * q_i . k_j;  softcap > 0: z = softcap * tanh(z / softcap);
+ *   slopes: z -= slopes[head] * |i + (nk - nq) - j|;
+ *   out_i = softmax over the visible keys (z) . v
+ * causal != 0: only keys j <= i + (nk - nq) are visible, and with prefix also the
+ * document's first prefix[d] keys.  A row without visible keys gets zeros; what
+ * invisible keys and values hold (NaN, infinities) has no influence.
+ * q, out: [q_rows][heads][head_dim]; k, v: [kv_rows][kv_heads][head_dim]; f16 or
+ * bf16, rows at the given strides (elements, multiples of 8), 16-byte
+ * aligned; head_dim 64 or 128; heads a multiple of kv_heads (query head h uses
+ * key head h / (heads / kv_heads)).  Softmax and sums in fp32, the
+ * probabilities rounded to the input type for the second product.
+ * Documents: q_offsets and kv_offsets [documents + 1] int32 (device,
+ * non-decreasing): document d has query rows [q_offsets[d], q_offsets[d + 1]) and
+ * the key slot [kv_offsets[d], kv_offsets[d + 1]); or both NULL: documents of
+ * q_len query rows each (documents * q_len == q_rows) with kv_len keys from row
+ * d * kv_pitch on.  kv_lengths [documents] (nullable): keys in use at the start of
+ * each slot.  Values outside the tensors are clamped to them.  Query rows
+ * outside every document are not written.
+ * out must not overlap q, k or v.  workspace: musc_b200_masked_attention_bytes
+ * (0 if none is needed), 256-byte aligned, free for reuse once the stream has
+ * passed the call. */
+typedef struct musc_b200_masked_attention_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int dtype, heads, kv_heads, head_dim;
+  long long q_rows, kv_rows;
+  long long q_stride, k_stride, v_stride, out_stride;
+  int documents;
+  int causal;
+  const int* q_offsets;
+  const int* kv_offsets;
+  const int* kv_lengths;
+  const int* prefix;
+  long long q_len, kv_len, kv_pitch;
+  const float* slopes;
+  float scale, softcap;
+  void* workspace;
+  size_t workspace_bytes;
+} musc_b200_masked_attention_args;
+
+/* Workspace of a call with these sizes (pointers are not looked at, except for
+ * q_offsets being NULL or not); 0 also for arguments that the call refuses. */
+size_t musc_b200_masked_attention_bytes(const musc_b200_masked_attention_args* args);
+
+int musc_b200_masked_attention(const musc_b200_masked_attention_args* args, musc_b200_stream stream);
 
 /* ------------------------------------------------------------------------
  * Pool-image preprocessing: the evaluation transform the reference applies to

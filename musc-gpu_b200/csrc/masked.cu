@@ -1,0 +1,177 @@
+// Entry point of masked attention (masked.cuh has the operator): checks, the choice of the
+// kernel and of the splits, and the kernel that joins the splits' partial sums.
+#include "masked.cuh"
+
+#include <string>
+
+namespace musc {
+namespace masked {
+namespace {
+
+// Joins the splits: out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m).  One
+// warp per (row, head); the partial outputs were just written and come out of L2.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (unit >= p.q_rows * p.heads) return;
+  const long long row = unit / p.heads;
+  const int head = (int)(unit - row * p.heads), lane = threadIdx.x & 31;
+  const int doc = find_document(p, row);
+  if (doc < 0) return;
+  const Interval iv = row_interval(p, doc, row);
+  const long long per_split = p.q_rows * p.heads;
+  float common = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) common = fmaxf(common, p.part_ml[s * per_split + unit].x);
+  common = warp_max(common);
+  float acc[D / 32], total = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = p.part_ml[s * per_split + unit];
+    const float w = split_weight(ml.x, common);
+    total = fmaf(w, ml.y, total);
+    if (w == 0.f && ml.y == 0.f) continue;  // nothing was written for it
+    const float* o = p.part + (s * per_split + unit) * D + lane * (D / 32);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, o[i], acc[i]);
+  }
+  const float inv = inverse_sum(total, iv.hi > iv.lo);
+  uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.out_stride + (long long)head * D + lane * (D / 32);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const float v = acc[i] * inv;
+    out[i] = FP16 ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+  }
+}
+
+}  // namespace
+
+int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t s) {
+  const unsigned grid = (unsigned)((p.q_rows * p.heads + 3) / 4);
+  if (head_dim == 64)
+    fp16 ? combine_kernel<64, true><<<grid, 128, 0, s>>>(p) : combine_kernel<64, false><<<grid, 128, 0, s>>>(p);
+  else
+    fp16 ? combine_kernel<128, true><<<grid, 128, 0, s>>>(p) : combine_kernel<128, false><<<grid, 128, 0, s>>>(p);
+  return check_launch("masked combine_kernel");
+}
+
+namespace {
+
+struct Plan {
+  int splits = 1;
+  size_t ml_offset = 0, bytes = 0;
+};
+
+// Keys that one document can have, as far as the host knows.
+long long kv_bound(const musc_b200_masked_attention_args& a) { return a.q_offsets ? a.kv_rows : a.kv_len; }
+
+Plan make_plan(const musc_b200_masked_attention_args& a) {
+  Plan plan;
+  const long long rows = a.q_rows * a.heads;
+  const int group = a.heads / a.kv_heads;
+  plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), kv_bound(a));
+  if (plan.splits > 1) {
+    plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;
+    plan.bytes = plan.ml_offset + (size_t)plan.splits * rows * sizeof(float2);
+  }
+  return plan;
+}
+
+int invalid(const char* what) { return fail(MUSC_B200_ERR_INVALID, std::string("masked_attention: ") + what); }
+
+int check_args(const musc_b200_masked_attention_args& a) {
+  if (a.dtype != MUSC_B200_F16 && a.dtype != MUSC_B200_BF16) return invalid("dtype must be f16 or bf16");
+  if (a.head_dim != 64 && a.head_dim != 128) return invalid("head_dim must be 64 or 128");
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads % a.kv_heads != 0 || a.heads > 4096)
+    return invalid("heads must be a multiple of kv_heads, both positive, at most 4096");
+  if (a.q_rows < 0 || a.kv_rows < 0 || a.q_rows > 0x7FFFFFFF - 256 || a.kv_rows > 0x7FFFFFFF - 256)
+    return invalid("q_rows and kv_rows must be below 2^31 - 256");
+  if (a.documents < 0) return invalid("documents must not be negative");
+  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return invalid("scale must be positive and finite");
+  if (!(a.softcap >= 0.f) || a.softcap > 3.0e38f) return invalid("softcap must be 0 (none) or positive and finite");
+  if (a.prefix && !a.causal) return invalid("a prefix needs causal");
+  if (a.q_offsets) {
+    if (!a.kv_offsets) return invalid("q_offsets and kv_offsets go together");
+  } else {
+    if (a.kv_offsets) return invalid("q_offsets and kv_offsets go together");
+    if (a.q_len < 0 || a.kv_len < 0 || a.kv_pitch < a.kv_len || a.q_len > a.q_rows || a.kv_pitch > 0x7FFFFFFF)
+      return invalid("0 <= q_len <= q_rows and 0 <= kv_len <= kv_pitch < 2^31");
+    if (a.q_len * a.documents != a.q_rows) return invalid("documents of q_len rows must make q_rows");
+    if (a.documents > 0 && (a.documents - 1) * a.kv_pitch + a.kv_len > a.kv_rows)
+      return invalid("the documents' key slots must lie within kv_rows");
+  }
+  return MUSC_B200_OK;
+}
+
+int check_tensors(const musc_b200_masked_attention_args& a) {
+  const long long qw = (long long)a.heads * a.head_dim, kw = (long long)a.kv_heads * a.head_dim;
+  if (!a.q || !a.out || (a.kv_rows > 0 && (!a.k || !a.v))) return invalid("null pointer");
+  if ((a.q_rows > 1 && (a.q_stride < qw || a.out_stride < qw)) || (a.kv_rows > 1 && (a.k_stride < kw || a.v_stride < kw)))
+    return invalid("row strides must hold all heads of a row");
+  for (long long s : {a.q_rows > 1 ? a.q_stride : 0, a.q_rows > 1 ? a.out_stride : 0, a.kv_rows > 1 ? a.k_stride : 0,
+                      a.kv_rows > 1 ? a.v_stride : 0})
+    if (s % 8 != 0 || s >= (1LL << 36)) return invalid("row strides must be multiples of 8 below 2^36");
+  for (const void* ptr : {a.q, a.k, a.v, (const void*)a.out})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0) return invalid("q, k, v and out must be 16-byte aligned");
+  // Byte ranges that a matrix spans: the output may share none of them.
+  const auto begin = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr); };
+  const auto end = [](const void* ptr, long long rows, long long stride, long long width) {
+    return reinterpret_cast<uintptr_t>(ptr) + (rows > 0 ? ((rows - 1) * stride + width) * 2 : 0);
+  };
+  const uintptr_t o0 = begin(a.out), o1 = end(a.out, a.q_rows, a.out_stride, qw);
+  if ((o0 < end(a.q, a.q_rows, a.q_stride, qw) && begin(a.q) < o1) ||
+      (o0 < end(a.k, a.kv_rows, a.k_stride, kw) && begin(a.k) < o1) ||
+      (o0 < end(a.v, a.kv_rows, a.v_stride, kw) && begin(a.v) < o1))
+    return invalid("out must not overlap q, k or v");
+  for (const void* ptr : {(const void*)a.q_offsets, (const void*)a.kv_offsets, (const void*)a.kv_lengths,
+                          (const void*)a.prefix, (const void*)a.slopes})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0) return invalid("offsets, lengths and slopes must be 4-byte aligned");
+  return MUSC_B200_OK;
+}
+
+}  // namespace
+}  // namespace masked
+}  // namespace musc
+
+using namespace musc;
+
+extern "C" size_t musc_b200_masked_attention_bytes(const musc_b200_masked_attention_args* args) {
+  if (!args || masked::check_args(*args) != MUSC_B200_OK || args->q_rows == 0 || args->documents == 0) return 0;
+  return masked::make_plan(*args).bytes;
+}
+
+extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args* args, musc_b200_stream stream) {
+  using namespace masked;
+  if (!args) return invalid("null arguments");
+  const musc_b200_masked_attention_args& a = *args;
+  MUSC_TRY(check_args(a));
+  if (a.q_rows == 0 || a.documents == 0) return MUSC_B200_OK;  // no row belongs to a document
+  MUSC_TRY(check_tensors(a));
+  const Plan plan = make_plan(a);
+  if (plan.bytes > 0) {
+    if (!a.workspace || a.workspace_bytes < plan.bytes)
+      return fail(MUSC_B200_ERR_WORKSPACE, "masked_attention: workspace smaller than musc_b200_masked_attention_bytes");
+    if (reinterpret_cast<uintptr_t>(a.workspace) % 256 != 0) return invalid("workspace must be 256-byte aligned");
+  }
+  MUSC_TRY(require_sm100());
+  Params p;
+  p.q = a.q, p.k = a.k, p.v = a.v, p.out = a.out;
+  p.q_stride = a.q_stride, p.k_stride = a.k_stride, p.v_stride = a.v_stride, p.out_stride = a.out_stride;
+  p.q_rows = a.q_rows, p.kv_rows = a.kv_rows;
+  p.q_offsets = a.q_offsets, p.kv_offsets = a.kv_offsets, p.kv_lengths = a.kv_lengths, p.prefix = a.prefix;
+  p.documents = a.documents;
+  p.q_len = a.q_len, p.kv_len = a.kv_len, p.kv_pitch = a.kv_pitch;
+  p.slopes = a.slopes;
+  p.heads = a.heads, p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads;
+  p.causal = a.causal, p.scale = a.scale, p.cap = a.softcap;
+  p.splits = plan.splits;
+  p.part = static_cast<float*>(a.workspace);
+  p.part_ml = plan.bytes ? reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.ml_offset) : nullptr;
+  p.err = device_error_ptr();
+  if (!p.err) return fail(MUSC_B200_ERR_CUDA, "masked_attention: device error word unavailable");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const bool fp16 = a.dtype == MUSC_B200_F16;
+  MUSC_TRY(rows_launch(p, a.head_dim, fp16, s));
+  if (plan.splits > 1) MUSC_TRY(combine_launch(p, a.head_dim, fp16, s));
+  return MUSC_B200_OK;
+}

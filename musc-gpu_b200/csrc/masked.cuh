@@ -1,0 +1,139 @@
+// Masked attention: what its kernels share.  For a query row i of a document with nq
+// queries and nk keys and a key j of the same document, in 32 bits,
+//
+//   z = scale * q_i . k_j;   z = cap * tanh(z / cap)          (cap > 0)
+//   z -= slope[head] * |i + (nk - nq) - j|                     (slopes given)
+//   out_i = sum_j exp(z_ij) v_j / sum_j exp(z_ij)              over the keys that row i sees
+//
+// A row sees no other document's keys; with `causal` only the keys up to its own position
+// i + (nk - nq), or the document's first prefix[d] keys where those reach further.  Every
+// one of these masks leaves a row one interval of the packed keys, which is all that the
+// kernels know of them.  A row that sees no key gets zeros.
+#pragma once
+
+#include "common.cuh"
+
+namespace musc {
+namespace masked {
+
+struct Params {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  long long q_stride, k_stride, v_stride, out_stride;  // elements between consecutive rows
+  long long q_rows, kv_rows;
+  // Documents: by offsets, or (q_offsets null) equal ones of q_len rows with key slots
+  // kv_pitch rows apart.
+  const int* q_offsets;
+  const int* kv_offsets;
+  const int* kv_lengths;  // null: a slot is used whole
+  const int* prefix;
+  int documents;
+  long long q_len, kv_len, kv_pitch;
+  const float* slopes;
+  int heads, kv_heads, group;  // group = heads / kv_heads
+  int causal;
+  float scale, cap;
+  // Keys split over `splits` CTAs: unnormalised partial outputs in 32 bits
+  // [split][row][head][head_dim] with each row's reference maximum and sum beside them.
+  int splits;
+  float* part;
+  float2* part_ml;
+  int* err;
+};
+
+// Keys [lo, hi) of the packed keys that a row sees, and the key its own position falls on.
+// lo is the first key of the row's document.  Whatever the offsets hold, 0 <= lo <= hi <= kv_rows.
+struct Interval {
+  long long lo, hi, pos;
+};
+
+// Document of a row: the last one that begins at or before it.  -1: the row belongs to none.
+__device__ __forceinline__ int find_document(const Params& p, long long row) {
+  if (!p.q_offsets) return (int)(row / p.q_len);
+  if (row < __ldg(p.q_offsets) || row >= __ldg(p.q_offsets + p.documents)) return -1;
+  int lo = 0, hi = p.documents;  // offsets[lo] <= row < offsets[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(p.q_offsets + mid) <= row) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ Interval row_interval(const Params& p, int doc, long long row) {
+  long long q0, nq, k0, nk;
+  if (p.q_offsets) {
+    q0 = __ldg(p.q_offsets + doc);
+    nq = __ldg(p.q_offsets + doc + 1) - q0;
+    k0 = min(max((long long)__ldg(p.kv_offsets + doc), 0LL), p.kv_rows);
+    nk = min(max((long long)__ldg(p.kv_offsets + doc + 1), k0), p.kv_rows) - k0;
+  } else {
+    q0 = doc * p.q_len;
+    nq = p.q_len;
+    k0 = doc * p.kv_pitch;
+    nk = p.kv_len;
+  }
+  if (p.kv_lengths) nk = min(max((long long)__ldg(p.kv_lengths + doc), 0LL), nk);
+  Interval r;
+  r.lo = k0;
+  r.pos = k0 + (row - q0) + (nk - nq);
+  long long seen = nk;
+  if (p.causal) {
+    seen = r.pos + 1 - k0;
+    if (p.prefix) seen = max(seen, (long long)__ldg(p.prefix + doc));
+    seen = min(max(seen, 0LL), nk);
+  }
+  r.hi = k0 + seen;
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// cap * tanh(x / cap) * log2(e) as cap2 - 2 cap2 / (1 + e^(2 x / cap)), cap2 = cap log2(e):
+// off by a few 2^-24 of cap2 for any x, which no 16-bit output sees.  two_over_cap2 is
+// 2 log2(e) / cap.
+__device__ __forceinline__ float capped_log2(float x, float two_over_cap2, float cap2) {
+  return fmaf(-2.f * cap2, rcp(1.f + ex2(x * two_over_cap2)), cap2);
+}
+
+// log2 by which the stored exponentials are raised.  In fp16 a weight below 2^-24 of the row's
+// largest would be lost; raised by 2^6 (and up to 2^8 more while a running maximum lags, still
+// below 65504) it keeps 2^-30.  Sums carry the same factor, which cancels.  bf16 has fp32's range.
+template <bool FP16>
+constexpr float RAISE = FP16 ? 6.f : 0.f;
+
+// Weight of a split's partial sums against the row's common maximum.
+__device__ __forceinline__ float split_weight(float m, float common) {
+  return m == -INFINITY ? 0.f : ex2(m - common);
+}
+
+// 1 / l of a finished row.  Sums of zero: a row without keys gets zeros, one whose every
+// visible score is -inf gets NaN, as 0 / 0.
+__device__ __forceinline__ float inverse_sum(float l, bool any_key) {
+  if (l == 0.f) return any_key ? NAN : 0.f;
+  return 1.f / l;
+}
+
+// Splits of the keys that give `units` CTAs of work enough CTAs (launchers of both kernels).
+int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
+int rows_splits(long long units, long long kv_bound);
+int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
+int tiles_splits(long long units, long long kv_bound);
+int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
+
+}  // namespace masked
+}  // namespace musc

@@ -16,10 +16,24 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().with_name('libmusc_b200.so')
 
 OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE, ERR_WORKSPACE, ERR_TIMEOUT = range(6)
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 BICUBIC, BILINEAR = 0, 1
 
 _vp, _ll, _int, _sz, _f = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_size_t, ctypes.c_float
+
+
+class MaskedAttentionArgs(ctypes.Structure):
+    """``musc_b200_masked_attention_args`` of include/musc_b200.h, field for field."""
+    _fields_ = [('q', _vp), ('k', _vp), ('v', _vp), ('out', _vp),
+                ('dtype', _int), ('heads', _int), ('kv_heads', _int), ('head_dim', _int),
+                ('q_rows', _ll), ('kv_rows', _ll),
+                ('q_stride', _ll), ('k_stride', _ll), ('v_stride', _ll), ('out_stride', _ll),
+                ('documents', _int), ('causal', _int),
+                ('q_offsets', _vp), ('kv_offsets', _vp), ('kv_lengths', _vp), ('prefix', _vp),
+                ('q_len', _ll), ('kv_len', _ll), ('kv_pitch', _ll),
+                ('slopes', _vp), ('scale', _f), ('softcap', _f),
+                ('workspace', _vp), ('workspace_bytes', _sz)]
+
 
 # name -> (restype, argtypes); the exact set declared in include/musc_b200.h.
 SIGNATURES = {
@@ -54,6 +68,11 @@ SIGNATURES = {
     'musc_b200_msm': (_int, [_vp, _int, _int, _int, _int, _int, _vp, _vp, _sz, _vp]),
     'musc_b200_attention_fwd': (_int, [_vp, _vp, _vp, _vp, _int, _int, _int, _int, _int, _ll, _ll, _f, _vp]),
     'musc_b200_add_layernorm': (_int, [_vp, _vp, _int, _vp, _vp, ctypes.c_float, _vp, _int, _ll, _int, _vp]),
+    'musc_b200_add_rmsnorm': (_int, [_vp, _int, _vp, _int, _vp, _f, _vp, _int, _vp, _int, _ll, _int, _ll, _ll, _ll, _vp]),
+    'musc_b200_rotary': (_int, [_vp, _vp, _vp, _vp, _int, _ll, _int, _int, _int, _ll, _ll, _ll, _ll, _vp, _int, _int, _vp,
+                                _vp, _int, _int, _vp]),
+    'musc_b200_masked_attention_bytes': (_sz, [ctypes.POINTER(MaskedAttentionArgs)]),
+    'musc_b200_masked_attention': (_int, [ctypes.POINTER(MaskedAttentionArgs), _vp]),
     'musc_b200_preprocess_workspace_bytes': (_sz, [_int, _int, _int, _int, _int]),
     'musc_b200_preprocess_images': (_int, [_vp, _int, _int, _int, _ll, _int, _int, _int,
                                            ctypes.POINTER(_f), ctypes.POINTER(_f), _int, _vp, _vp, _sz, _vp]),

@@ -509,6 +509,265 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     return out
 
 
+def _forward_only(what: str, *tensors: torch.Tensor | None) -> None:
+    """These operators have no backward pass: refuse inputs whose gradient would be lost."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f'{what}: no gradient is computed; call it under torch.no_grad() or detach the inputs')
+
+
+def _on_device(what: str, device: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f'{what}: {name} must be on {device}')
+
+
+def _token_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    """``(rows, row stride, rows between batch items)`` of a token-major ``(T, W)`` or ``(B, L, W)`` tensor."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f'{what}: {name} must be contiguous in its last dimension')
+    if t.ndim == 2:
+        return t.shape[0], (t.stride(0) if t.shape[0] > 1 else t.shape[1]), t.shape[0]
+    b, length, width = t.shape
+    if b * length == 0:
+        return 0, width, length
+    if length == 1:
+        return b, (t.stride(0) if b > 1 else width), 1
+    if b == 1:
+        return length, t.stride(1), length
+    if t.stride(1) <= 0 or t.stride(0) % t.stride(1) != 0 or t.stride(0) // t.stride(1) < length:
+        raise ValueError(f'{what}: the batch items of {name} must lie a whole number of rows apart')
+    pitch = t.stride(0) // t.stride(1)
+    return (b - 1) * pitch + length, t.stride(1), pitch
+
+
+def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: int | None = None, *,
+                     offsets: torch.Tensor | None = None, kv_offsets: torch.Tensor | None = None,
+                     kv_lengths: torch.Tensor | None = None, causal: bool = False,
+                     prefix: torch.Tensor | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention within documents: packed images or texts of differing lengths, padded batches, or new
+    tokens against a cache.
+
+    ``q`` ``(T, heads*D)`` and ``k``, ``v`` ``(S, kv_heads*D)`` (fp16 or bf16, D 64 or 128, columns of one
+    projection allowed) with ``offsets`` ``(docs + 1,)`` int32 on the device: document ``d`` has the query
+    rows ``[offsets[d], offsets[d+1])`` and the key slot ``[kv_offsets[d], kv_offsets[d+1])``
+    (``kv_offsets`` defaults to ``offsets``).  Or ``q`` ``(B, L, heads*D)`` and ``k``, ``v``
+    ``(B, S, kv_heads*D)`` without offsets: each batch item is a document.  ``kv_lengths`` ``(docs,)`` int32:
+    the keys in use at the start of each slot.
+
+    Query ``i`` of a document with ``nq`` queries and ``nk`` keys stands at key position ``i + nk - nq``.
+    It sees the document's keys, with ``causal`` only those up to its position, and with ``prefix``
+    ``(docs,)`` int32 also the first ``prefix[d]`` ones.  Scores are ``scale * q.k`` (``D**-0.5``), capped as
+    ``softcap * tanh(z / softcap)`` if ``softcap > 0``, less ``slopes[head] * distance`` with ``slopes``
+    ``(heads,)`` fp32.  A row that sees no key gives zeros; rows outside every document are left as they
+    are (of a fresh output: undefined).  Forward only.
+    """
+    what = 'attention_masked'
+    _require_cuda(q, what)
+    _forward_only(what, q, k, v, slopes)
+    dev = q.device
+    _on_device(what, dev, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, kv_lengths=kv_lengths, prefix=prefix,
+               slopes=slopes, out=out)
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError('attention_masked: q, k, v must all be float16 or all bfloat16')
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads != 0 or q.shape[-1] % heads != 0:
+        raise ValueError('attention_masked: heads must be a multiple of kv_heads and divide the width of q')
+    head_dim = q.shape[-1] // heads
+    packed = offsets is not None
+    if q.ndim != (2 if packed else 3) or k.ndim != q.ndim or k.shape != v.shape or k.shape[-1] != kv_heads * head_dim:
+        raise ValueError('attention_masked: expected q (T, heads*D), k and v (S, kv_heads*D) with offsets, '
+                         'or q (B, L, heads*D), k and v (B, S, kv_heads*D) without')
+    if packed:
+        kv_offsets = offsets if kv_offsets is None else kv_offsets
+        docs = offsets.numel() - 1
+    else:
+        if kv_offsets is not None:
+            raise ValueError('attention_masked: kv_offsets needs offsets')
+        if k.shape[0] != q.shape[0]:
+            raise ValueError('attention_masked: q, k, v must have the same batch')
+        docs = q.shape[0]
+    for name, t, n, dtype in (('offsets', offsets, docs + 1, torch.int32), ('kv_offsets', kv_offsets, docs + 1, torch.int32),
+                              ('kv_lengths', kv_lengths, docs, torch.int32), ('prefix', prefix, docs, torch.int32),
+                              ('slopes', slopes, heads, torch.float32)):
+        if t is not None and (t.dtype != dtype or t.shape != (n,) or not t.is_contiguous() or n < 0 or docs < 0):
+            raise ValueError(f'attention_masked: {name} must be a contiguous ({n},) {dtype} tensor')
+    q_rows, q_stride, q_pitch = _token_rows(what, 'q', q)
+    kv_rows, k_stride, kv_pitch = _token_rows(what, 'k', k)
+    _, v_stride, v_pitch = _token_rows(what, 'v', v)
+    if q.ndim == 3 and (q_pitch != q.shape[1] or v_pitch != kv_pitch):
+        raise ValueError('attention_masked: batch items of q must follow each other, those of k and v lie equally far apart')
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError('attention_masked: out must have the shape and type of q')
+    _, out_stride, out_pitch = _token_rows(what, 'out', out)
+    if q.ndim == 3 and out_pitch != q_pitch:
+        raise ValueError('attention_masked: batch items of out must follow each other')
+    args = _lib.MaskedAttentionArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), dtype=_DTYPES[q.dtype], heads=heads,
+        kv_heads=kv_heads, head_dim=head_dim, q_rows=q_rows, kv_rows=kv_rows, q_stride=q_stride, k_stride=k_stride,
+        v_stride=v_stride, out_stride=out_stride, documents=docs, causal=int(causal),
+        q_offsets=offsets.data_ptr() if packed else None, kv_offsets=kv_offsets.data_ptr() if packed else None,
+        kv_lengths=kv_lengths.data_ptr() if kv_lengths is not None else None,
+        prefix=prefix.data_ptr() if prefix is not None else None,
+        q_len=0 if packed else q.shape[1], kv_len=0 if packed else k.shape[1], kv_pitch=0 if packed else kv_pitch,
+        slopes=slopes.data_ptr() if slopes is not None else None,
+        scale=head_dim ** -0.5 if scale is None else scale, softcap=softcap)
+    lib = _lib.lib()
+    with torch.cuda.device(dev):
+        ws_bytes = lib.musc_b200_masked_attention_bytes(ctypes.byref(args))
+        if ws_bytes:
+            ws = _aligned_empty(ws_bytes, dev, 256)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
+        st = lib.musc_b200_masked_attention(ctypes.byref(args), _stream(dev))
+        _lib.check(st, 'musc_b200_masked_attention')
+    return out
+
+
+# --------------------------------------------------------------------------- rotary positions
+def rotary_frequencies(sections: Sequence[int], base: float = 10000.0, shared: bool = False,
+                       device='cuda') -> tuple[torch.Tensor, torch.Tensor]:
+    """``(frequencies fp32, axis int32)`` for :func:`rotary`: ``sections[a]`` pairs turn with axis ``a``.
+
+    Each axis has its own ladder ``base ** (-i / sections[a])``, or (``shared``) the axes take
+    consecutive parts of one ladder ``base ** (-i / sum(sections))``.
+    """
+    sections = [int(n) for n in sections]
+    if not sections or min(sections) < 0 or sum(sections) <= 0:
+        raise ValueError('rotary_frequencies: sections must be pairs per axis')
+    total = sum(sections)
+    if shared:
+        exponents = [i / total for i in range(total)]
+    else:
+        exponents = [i / n for n in sections for i in range(n)]
+    frequencies = torch.tensor([base ** -e for e in exponents], dtype=torch.float64).float()
+    axis = torch.tensor([a for a, n in enumerate(sections) for _ in range(n)], dtype=torch.int32)
+    return frequencies.to(device), axis.to(device)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: torch.Tensor,
+           axis: torch.Tensor, heads: int, kv_heads: int | None = None, adjacent: bool = False,
+           out: tuple[torch.Tensor, torch.Tensor | None] | None = None):
+    """Rotary positions over several axes: pair ``p`` of every head turns by
+    ``positions[..., axis[p]] * frequencies[p]`` radians; returns the turned ``(q, k)``.
+
+    ``q`` ``(..., heads*D)``, ``k`` ``(..., kv_heads*D)`` (or None) in fp32, fp16 or bf16, ``(T, W)`` or
+    ``(B, L, W)``, columns of one projection allowed; ``positions`` ``(..., axes)`` int32 or fp32, e.g. (time,
+    row, column); ``frequencies`` fp32 and ``axis`` int32 of the turned pairs
+    (:func:`rotary_frequencies`).  Pairs are dims ``(p, p + pairs)``, or ``(2p, 2p + 1)`` if
+    ``adjacent``; dims past ``2 * pairs`` are copied.  ``out=(q, k)`` turns them in place.  Forward only.
+    """
+    what = 'rotary'
+    _require_cuda(q, what)
+    _forward_only(what, q, k, positions, frequencies)
+    dev = q.device
+    outs = (None, None) if out is None else out
+    _on_device(what, dev, k=k, positions=positions, frequencies=frequencies, axis=axis, q_out=outs[0], k_out=outs[1])
+    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+        raise ValueError('rotary: q and k must share one type, float32, float16 or bfloat16')
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or q.shape[-1] % heads != 0:
+        raise ValueError('rotary: heads must divide the width of q')
+    head_dim = q.shape[-1] // heads
+    if q.ndim not in (2, 3) or (k is not None and k.shape != (*q.shape[:-1], kv_heads * head_dim)):
+        raise ValueError('rotary: expected q (T, heads*D) or (B, L, heads*D) and k (..., kv_heads*D) of as many tokens')
+    if positions.dtype not in (torch.int32, torch.float32) or positions.ndim != q.ndim or \
+            positions.shape[:-1] != q.shape[:-1] or positions.shape[-1] < 1 or not positions.is_contiguous():
+        raise ValueError('rotary: positions must be a contiguous (..., axes) int32 or float32 tensor with the tokens of q')
+    if frequencies.dtype != torch.float32 or frequencies.ndim != 1 or not frequencies.is_contiguous():
+        raise ValueError('rotary: frequencies must be a contiguous (pairs,) float32 tensor')
+    if axis.dtype != torch.int32 or axis.shape != frequencies.shape or not axis.is_contiguous():
+        raise ValueError('rotary: axis must be a contiguous int32 tensor of the shape of frequencies')
+    ins = [q] if k is None else [q, k]
+    if out is None:
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in ins]
+    else:
+        outs = list(out)[:len(ins)]
+        for t, o in zip(ins, outs):
+            if o is None or o.shape != t.shape or o.dtype != t.dtype:
+                raise ValueError('rotary: out must be (q_out, k_out) of the shapes and type of q and k')
+    strides = []
+    for name, t in zip(('q', 'k', 'q_out', 'k_out') if k is not None else ('q', 'q_out'), ins + outs):
+        rows, stride, pitch = _token_rows(what, name, t)
+        if t.ndim == 3 and pitch != t.shape[1]:
+            raise ValueError(f'rotary: batch items of {name} must follow each other')
+        strides.append(stride)
+    tokens = q.numel() // q.shape[-1] if q.shape[-1] else 0
+    n = len(ins)
+    with torch.cuda.device(dev):
+        st = _lib.lib().musc_b200_rotary(
+            _ptr(q), _ptr(k), _ptr(outs[0]), _ptr(outs[1] if n == 2 else None), _DTYPES[q.dtype], tokens, heads,
+            kv_heads if n == 2 else 0, head_dim, strides[0], strides[1] if n == 2 else 0, strides[n],
+            strides[n + 1] if n == 2 else 0, _ptr(positions), int(positions.dtype == torch.float32),
+            positions.shape[-1], _ptr(frequencies), _ptr(axis), frequencies.numel(), int(adjacent), _stream(dev))
+        _lib.check(st, 'musc_b200_rotary')
+    return outs[0], (outs[1] if n == 2 else None)
+
+
+# --------------------------------------------------------------------------- RMS norm
+def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-6,
+                out_dtype: torch.dtype = torch.float16, group: int = 0, out: torch.Tensor | None = None,
+                scales: torch.Tensor | None = None):
+    """``x += delta`` in place (skipped when ``delta`` is None), then ``x / sqrt(mean(x^2) + eps) * weight``:
+    the residual add and root-mean-square norm of a block in one pass.
+
+    ``x`` ``(..., C)`` fp32, fp16 or bf16, ``delta`` of its shape in any of these types, ``weight`` ``(C,)``
+    fp32; both contiguous, or ``(rows, C)`` with rows a stride apart.  The sum is normalised in fp32 before
+    it is rounded to ``x``'s type.  Returns the result in ``out_dtype`` (fp32, fp16, bf16); for
+    ``torch.float8_e4m3fn`` returns ``(values, scales)`` with ``values * scales`` the result and one fp32
+    scale for each row (``group`` 0; ``scales`` ``(..., 1)``) or each ``group`` of 32, 64, 128 or 256 columns
+    (``(..., ceil(C / group))``).  Forward only.
+    """
+    what = 'add_rmsnorm'
+    _require_cuda(x, what)
+    _forward_only(what, x, delta, weight)
+    dev = x.device
+    _on_device(what, dev, delta=delta, weight=weight, out=out, scales=scales)
+    if x.ndim < 1 or x.dtype not in _DTYPES:
+        raise ValueError('add_rmsnorm: x must be float32, float16 or bfloat16 (..., C)')
+    if delta is not None and (delta.shape != x.shape or delta.dtype not in _DTYPES):
+        raise ValueError('add_rmsnorm: delta must be a float32, float16 or bfloat16 tensor of x\'s shape')
+    c = x.shape[-1]
+    rows = x.numel() // c if c else 0
+    if weight.dtype != torch.float32 or weight.shape != (c,) or not weight.is_contiguous():
+        raise ValueError('add_rmsnorm: weight must be a contiguous (C,) float32 tensor')
+    eight = out_dtype == torch.float8_e4m3fn
+    if out_dtype not in _DTYPES and not eight:
+        raise ValueError('add_rmsnorm: out_dtype must be float32, float16, bfloat16 or float8_e4m3fn')
+    if group not in (0, 32, 64, 128, 256) or (group and not eight):
+        raise ValueError('add_rmsnorm: group must be 0, or 32, 64, 128 or 256 for a float8_e4m3fn output')
+    if out is None:
+        out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+    if out.shape != x.shape or out.dtype != out_dtype:
+        raise ValueError('add_rmsnorm: out must have the shape of x and type out_dtype')
+    if eight:
+        shape = (*x.shape[:-1], -(-c // group) if group else 1)
+        if scales is None:
+            scales = torch.empty(shape, dtype=torch.float32, device=dev)
+        if scales.shape != shape or scales.dtype != torch.float32 or not scales.is_contiguous():
+            raise ValueError(f'add_rmsnorm: scales must be a contiguous {tuple(shape)} float32 tensor')
+    elif scales is not None:
+        raise ValueError('add_rmsnorm: scales are of a float8_e4m3fn output')
+    strides = []
+    for name, t in (('x', x), ('delta', delta), ('out', out)):
+        if t is None:
+            strides.append(c)
+        elif t.is_contiguous():
+            strides.append(c)
+        elif t.ndim == 2 and (t.stride(1) == 1 or c == 1):
+            strides.append(t.stride(0))
+        else:
+            raise ValueError(f'add_rmsnorm: {name} must be contiguous, or (rows, C) with contiguous rows')
+    with torch.cuda.device(dev):
+        st = _lib.lib().musc_b200_add_rmsnorm(
+            _ptr(x), _DTYPES[x.dtype], _ptr(delta), _DTYPES[delta.dtype] if delta is not None else 0, _ptr(weight),
+            float(eps), _ptr(out), _lib.E4M3 if eight else _DTYPES[out_dtype], _ptr(scales if eight else None), group,
+            rows, c, strides[0], strides[1], strides[2], _stream(dev))
+        _lib.check(st, 'musc_b200_add_rmsnorm')
+    return (out, scales) if eight else out
+
+
 OPENAI_MEAN = (0.48145466, 0.4578275, 0.40821073)
 OPENAI_STD = (0.26862954, 0.26130258, 0.27577711)
 _FILTERS = {'bicubic': _lib.BICUBIC, 'bilinear': _lib.BILINEAR}
