@@ -439,8 +439,8 @@ int encode_fn(EncodeTiledFn* fn) {
   return MUSC_B200_OK;
 }
 
-// bf16 [rows][row_stride] with the head slices as the inner dimension; box = one head
-// (64 elements = 128 bytes) x 128 token rows, 128-byte swizzle.
+}  // namespace
+
 int make_token_map(CUtensorMap* map, const void* base, long long rows, int inner, long long row_stride,
                    bool fp16) {
   EncodeTiledFn encode;
@@ -458,7 +458,6 @@ int make_token_map(CUtensorMap* map, const void* base, long long rows, int inner
   return MUSC_B200_OK;
 }
 
-}  // namespace
 }  // namespace musc
 
 using namespace musc;

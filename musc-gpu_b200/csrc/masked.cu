@@ -58,6 +58,7 @@ int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t s) {
 namespace {
 
 struct Plan {
+  bool tiles = false;
   int splits = 1;
   size_t ml_offset = 0, bytes = 0;
 };
@@ -69,7 +70,13 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   Plan plan;
   const long long rows = a.q_rows * a.heads;
   const int group = a.heads / a.kv_heads;
-  plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), kv_bound(a));
+  // A CTA of the tile kernel takes 256 rows of one head, one of the row kernel one row of all
+  // heads of a key head (up to 16), reading its keys again for every row.
+  plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
+  if (plan.tiles)
+    plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, kv_bound(a));
+  else
+    plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), kv_bound(a));
   if (plan.splits > 1) {
     plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;
     plan.bytes = plan.ml_offset + (size_t)plan.splits * rows * sizeof(float2);
@@ -171,7 +178,7 @@ extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args*
   if (!p.err) return fail(MUSC_B200_ERR_CUDA, "masked_attention: device error word unavailable");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool fp16 = a.dtype == MUSC_B200_F16;
-  MUSC_TRY(rows_launch(p, a.head_dim, fp16, s));
+  MUSC_TRY(plan.tiles ? tiles_launch(p, a.head_dim, fp16, s) : rows_launch(p, a.head_dim, fp16, s));
   if (plan.splits > 1) MUSC_TRY(combine_launch(p, a.head_dim, fp16, s));
   return MUSC_B200_OK;
 }
