@@ -442,12 +442,12 @@ int encode_fn(EncodeTiledFn* fn) {
 }  // namespace
 
 int make_token_map(CUtensorMap* map, const void* base, long long rows, int inner, long long row_stride,
-                   bool fp16) {
+                   bool fp16, int box_rows) {
   EncodeTiledFn encode;
   MUSC_TRY(encode_fn(&encode));
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)row_stride * 2};
-  cuuint32_t box[2] = {(cuuint32_t)attn::D, (cuuint32_t)attn::BKV};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = encode(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
                       const_cast<void*>(base), dims, strides, box,

@@ -10,7 +10,8 @@
 //                   sum in 32 bits, P rounded to 16 bits back into tensor memory over S;
 //   warp 8          TMA: Q once, K and V tiles through a ring;
 //   warp 9          one thread issues tcgen05.mma: S_h = Q_h K^T (128 x 128 x D, both from
-//                   shared memory) and O_h += P_h V (128 x D x 128, P from tensor memory).
+//                   shared memory) and O_h += P_h V (128 x D x 128, P from tensor memory);
+//   warp 10         zeroes the end of V's tiles that reach past their keys.
 // While one half's softmax runs, the tensor cores work for the other: the exponentials
 // (16 a cycle and SM: 1024 cycles for 128 x 128) bound the kernel for D = 64 (256 cycles of
 // products at the tensor cores' rate) and for D = 128 (512).  O stays in tensor memory and is
@@ -32,31 +33,31 @@ namespace {
 
 constexpr int BQ = 128;    // query rows of a half (TMEM lanes)
 constexpr int ROWS = 2 * BQ;
-constexpr int BKV = 128;   // keys of a tile
-constexpr int BLOCK_BYTES = 128 * 128;  // 128 rows x 64 elements, one swizzle block
+constexpr int BKV = 64;    // keys of a tile
+constexpr int Q_BLOCK = BQ * 128, KV_BLOCK = BKV * 128;  // bytes of 64 elements (a swizzle row) of all rows
 constexpr int SOFTMAX_WARPS = 8;
-constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);  // three warpgroups; two warps of the last idle
-// Registers of a thread: 168 at launch (65536 / 384), of which the copying and issuing
-// warpgroup gives back what the softmax ones take: 2 x 208 + 88 = 3 x 168.
-constexpr int SOFTMAX_REGS = 208, OTHER_REGS = 88;
+constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);  // the last warp is idle
 constexpr int TMEM_COLS = 512;
-constexpr int S_COL = 0;     // S (and P over its first half) at columns 0 and 128
-constexpr int O_COL = 256;   // O at columns 256 and 256 + D
-constexpr float RESCALE = 8.f;
+// Tensor memory: per half S (64 columns), two buffers of P (32 each) and O (D).
+constexpr int s_col(int h) { return h * 64; }
+constexpr int p_col(int h, int buffer) { return 128 + h * 64 + buffer * 32; }
+template <int D> constexpr int o_col(int h) { return 256 + h * D; }
+constexpr float P_LIMIT = 65504.f;  // largest sum of a row's stored exponentials over a tile: each fits fp16
 constexpr int SHARED_DOCS = 1024;  // offsets searched in shared memory up to this many documents
 constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-
-template <int D> constexpr int STAGES = D == 64 ? 4 : 2;
+constexpr uint32_t SLEEP_NS = 1000000;
+template <int D> constexpr int STAGES = D == 64 ? 8 : 4;
 
 template <int D>
 struct Smem {
-  uint8_t q[2][D / 64][BLOCK_BYTES];
-  uint8_t k[STAGES<D>][D / 64][BLOCK_BYTES];
-  uint8_t v[STAGES<D>][D / 64][BLOCK_BYTES];
+  uint8_t q[2][D / 64][Q_BLOCK];
+  uint8_t k[STAGES<D>][D / 64][KV_BLOCK];
+  uint8_t v[STAGES<D>][D / 64][KV_BLOCK];
   uint64_t q_full;
   uint64_t k_full[STAGES<D>], k_empty[STAGES<D>];
-  uint64_t v_full[STAGES<D>], v_empty[STAGES<D>];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t v_full[STAGES<D>], v_clean[STAGES<D>], v_empty[STAGES<D>];
+  uint64_t s_full[2], s_free[2];        // per half
+  uint64_t p_full[2][2], o_full[2][2];  // per half and buffer of P
   uint64_t drain;
   union {
     int offsets[SHARED_DOCS + 1];  // while the rows' documents are looked up
@@ -71,28 +72,50 @@ struct Smem {
 };
 template <int D> constexpr size_t SMEM_BYTES = sizeof(Smem<D>) + 1024;
 
+// Bounded wait.  The thread sleeps in try_wait (a warp that polled instead took up to 40 % of
+// its scheduler from the softmax warps there); the clock is read only after it has slept.
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  if (tc::mbar_try_wait(bar, parity)) return true;
+  if (tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) return true;
   const uint64_t start = global_ns();
-  uint32_t iter = 0;
-  while (true) {
-    if (tc::mbar_try_wait(bar, parity)) return true;
-    if ((++iter & 255u) == 0) {
-      if (*abort_flag) return false;
-      if (global_ns() - start > WAIT_LIMIT_NS) {
-        *abort_flag = 1;
-        atomicExch(err, MUSC_B200_ERR_TIMEOUT);
-        return false;
-      }
+  while (!tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) {
+    if (*abort_flag) return false;
+    if (global_ns() - start > WAIT_LIMIT_NS) {
+      *abort_flag = 1;
+      atomicExch(err, MUSC_B200_ERR_TIMEOUT);
+      return false;
     }
   }
+  return true;
 }
 
-// V as the MN-major B operand in the 128-byte swizzle: 8-key groups 1024 bytes apart, blocks of
-// 64 dims BLOCK_BYTES apart.
-__device__ __forceinline__ uint64_t desc_v(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(BLOCK_BYTES >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Shared-memory matrix descriptors in the 128-byte swizzle, 8-row groups 1024 bytes apart.  The
+// upper word is the same for every operand here; the lower one holds the address, so the
+// operands of consecutive products are an addition apart.  K-major (Q, K) has no leading
+// offset; V as the MN-major B operand has its blocks of 64 dims KV_BLOCK apart.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo_k(uint32_t smem_addr) { return (smem_addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_v(uint32_t smem_addr) {
+  return (smem_addr >> 4) | ((uint32_t)(KV_BLOCK >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"(DESC_HI)
+      : "memory");
+}
+// A (one row per TMEM lane) from tensor memory: a 32-bit column holds two consecutive K
+// elements, so a K step of 16 is eight columns.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"(DESC_HI)
+      : "memory");
 }
 template <bool FP16> constexpr uint32_t idesc_qk() { return tc::idesc_f16(BQ, BKV, FP16 ? 0 : 1); }
 template <int D, bool FP16> constexpr uint32_t idesc_pv() {
@@ -114,28 +137,112 @@ __device__ __forceinline__ float widen(uint16_t v) {
   return FP16 ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
 }
 
-// The tiles [first, first + left) of the CTA's walk over its segments.
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// The value, as one that changes from use to use: what is computed from it stays where it is used
+// instead of taking registers through the whole loop.
+__device__ __forceinline__ float here(float v) {
+  asm volatile("" : "+f"(v));
+  return v;
+}
+
+// s -> cap2 * tanh(s / cap) for a row's tile (factor = scale / cap, cap2 = cap log2(e)).  The exact form
+// takes two of the special-function unit's operations an element, and the exponential a
+// third: 3072 cycles a half's tile where the unit bounds the kernel.  tanh(x) / x as a
+// polynomial in x^2 takes multiply-adds instead, two elements an instruction: of degree 3
+// where the warp's scores stay within |x| <= 0.4 (most do: a cap is chosen well above them),
+// of degree 6 up to 1, each fitted for the least maximum error (2e-8 and 2e-8 of tanh, below
+// the rounding of its evaluation).
+__device__ __forceinline__ void cap_scores(float2 (&s)[BKV / 2], float factor_, float cap2_) {
+  const float factor = here(factor_), cap2 = here(cap2_);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < BKV / 2; ++i) top = max3(top, fabsf(s[i].x), fabsf(s[i].y));
+  const float x_max = top * factor;
+  if (__all_sync(0xffffffffu, x_max <= 0.4f)) {
+    const float2 c0 = both(cap2 * 0.999999583f), c1 = both(cap2 * -0.333297253f), c2 = both(cap2 * 0.13250567f),
+                 c3 = both(cap2 * -0.0468257405f);
+#pragma unroll
+    for (int i = 0; i < BKV / 2; ++i) {
+      const float2 x = mul2(s[i], both(factor)), t = mul2(x, x);
+      s[i] = mul2(x, fma2(fma2(fma2(c3, t, c2), t, c1), t, c0));
+    }
+  } else if (__all_sync(0xffffffffu, x_max <= 1.f)) {
+    const float2 c0 = both(cap2 * 0.999999702f), c1 = both(cap2 * -0.333321303f), c2 = both(cap2 * 0.133195832f),
+                 c3 = both(cap2 * -0.0532658361f), c4 = both(cap2 * 0.0199732818f), c5 = both(cap2 * -0.00595127977f),
+                 c6 = both(cap2 * 0.000963771949f);
+#pragma unroll
+    for (int i = 0; i < BKV / 2; ++i) {
+      const float2 x = mul2(s[i], both(factor)), t = mul2(x, x);
+      s[i] = mul2(x, fma2(fma2(fma2(fma2(fma2(fma2(c6, t, c5), t, c4), t, c3), t, c2), t, c1), t, c0));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < BKV / 2; ++i) {
+      s[i].x = capped_log2(s[i].x, 2.f * LOG2E * factor, cap2);
+      s[i].y = capped_log2(s[i].y, 2.f * LOG2E * factor, cap2);
+    }
+  }
+}
+
+// The tiles [first, last) of the CTA's walk over its segments, one segment's end in a register.
 struct Walk {
   const int2* segments;
-  int segment, x, left;
-  __device__ Walk(const int2* s, int first, int last) : segments(s), segment(0), left(last - first) {
+  int segment, x, stop, left;
+  __device__ __forceinline__ Walk(const int2* s, int first, int last) : segments(s), segment(0), left(last - first) {
+    x = stop = 0;
     while (left > 0) {
       const int tiles = (s[segment].y - s[segment].x + BKV - 1) / BKV;
       if (first < tiles) break;
       first -= tiles;
       ++segment;
     }
-    x = left > 0 ? s[segment].x + first * BKV : 0;
+    if (left > 0) x = s[segment].x + first * BKV, stop = s[segment].y;
   }
   // Next tile: keys [begin, end), end - begin <= BKV.
-  __device__ bool next(int& begin, int& end) {
+  __device__ __forceinline__ bool next(int& begin, int& end) {
     if (left <= 0) return false;
     --left;
     begin = x;
-    const int stop = segments[segment].y;
     end = min(x + BKV, stop);
     x += BKV;
-    if (x >= stop && left > 0) x = segments[++segment].x;
+    if (x >= stop && left > 0) {
+      const int2 s = segments[++segment];
+      x = s.x, stop = s.y;
+    }
     return true;
   }
 };
@@ -198,7 +305,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int NB = D / 64;
   constexpr int NS = STAGES<D>;
-  constexpr uint32_t TILE_BYTES = NB * BLOCK_BYTES;
+  constexpr uint32_t TILE_BYTES = NB * KV_BLOCK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &sm.abort_flag;
   // Heads change fastest (those of a group share K and V in L2), then the row tiles -- the
@@ -217,12 +324,16 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
       tc::mbar_init(tc::smem_u32(&sm.k_full[s]), 1);
       tc::mbar_init(tc::smem_u32(&sm.k_empty[s]), 1);
       tc::mbar_init(tc::smem_u32(&sm.v_full[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.v_clean[s]), 1);
       tc::mbar_init(tc::smem_u32(&sm.v_empty[s]), 1);
     }
     for (int h = 0; h < 2; ++h) {
       tc::mbar_init(tc::smem_u32(&sm.s_full[h]), 1);
-      tc::mbar_init(tc::smem_u32(&sm.p_full[h]), SOFTMAX_WARPS / 2);
-      tc::mbar_init(tc::smem_u32(&sm.o_full[h]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.s_free[h]), SOFTMAX_WARPS / 2);
+      for (int b = 0; b < 2; ++b) {
+        tc::mbar_init(tc::smem_u32(&sm.p_full[h][b]), SOFTMAX_WARPS / 2);
+        tc::mbar_init(tc::smem_u32(&sm.o_full[h][b]), 1);
+      }
     }
     tc::mbar_init(tc::smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
@@ -323,12 +434,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   const auto needs = [&](int h, int begin, int end) { return begin < sm.hull[h][1] && end > sm.hull[h][0]; };
 
   if (warp >= SOFTMAX_WARPS) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
    if (warp == SOFTMAX_WARPS) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && n_tiles > 0) {
       const uint32_t qf = tc::smem_u32(&sm.q_full);
-      tc::mbar_arrive_expect_tx(qf, 2 * TILE_BYTES);
+      tc::mbar_arrive_expect_tx(qf, 2 * NB * Q_BLOCK);
       for (int h = 0; h < 2; ++h)
         for (int b = 0; b < NB; ++b)
           tc::tma_load_2d(tc::smem_u32(sm.q[h][b]), &map_q, head * D + b * 64, (int)row0 + h * BQ, qf);
@@ -365,151 +475,166 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
       }
     }
    } else if (warp == SOFTMAX_WARPS + 1) {
-    // ------------------------------------------------------------ MMA issuer (the warp stays together)
-    if (n_tiles > 0) {
+    // ------------------------------------------------------------ MMA issuer: one thread, and
+    // little code, since the softmax warps' loops keep it out of the instruction caches
+    if (n_tiles > 0 && tc::elect_one()) {
       Walk walk(sm.segments, first_tile, last_tile);
-      int begin = 0, end = 0, next_begin = 0, next_end = 0;
-      int sequence[2] = {0, 0};          // tiles of each half so far
-      bool pending[2] = {false, false};  // a P V product of the half that no one has waited for
-      const auto issue_qk = [&](int h, int s) {
-        if (lane == 0) {
-          const uint32_t q_addr = tc::smem_u32(sm.q[h][0]), k_addr = tc::smem_u32(sm.k[s][0]);
-          const uint32_t d_tmem = tmem_base + (uint32_t)(S_COL + h * BKV);
-#pragma unroll
-          for (int t = 0; t < D / 16; ++t) {
-            const uint32_t at = (uint32_t)((t >> 2) * BLOCK_BYTES + (t & 3) * 32);
-            tc::mma_f16_ss(d_tmem, tc::desc_k_sw128(q_addr + at), tc::desc_k_sw128(k_addr + at), idesc_qk<FP16>(),
-                           t ? 1u : 0u);
-          }
-          tc::mma_commit(tc::smem_u32(&sm.s_full[h]));
-        }
-        __syncwarp();
+      int begin = 0, end = 0;
+      // Products of each half so far (S and P V), and whether the half needs this tile and the next.
+      uint32_t scores[2] = {0, 0}, outputs[2] = {0, 0};
+      bool ok = true, needed[2], next[2];
+      const uint32_t q_lo = desc_lo_k(tc::smem_u32(sm.q)), k_lo = desc_lo_k(tc::smem_u32(sm.k));
+      const uint32_t v_lo = desc_lo_v(tc::smem_u32(sm.v));
+      const auto await = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag, p.err);
       };
-      bool ok = wait_bounded(tc::smem_u32(&sm.q_full), 0, abort_flag, p.err) &&
-                wait_bounded(tc::smem_u32(&sm.k_full[0]), 0, abort_flag, p.err);
-      ok = __all_sync(0xffffffffu, ok);
-      walk.next(begin, end);
-      if (ok) {
+      // S of half h for the tile in stage s, once the softmax has read the S before.
+      const auto issue_qk = [&](int h, int s) {
+        if (scores[h] > 0) await(&sm.s_free[h], scores[h] - 1);
+        if (!ok) return;
         tc::fence_after_sync();
-        for (int h = 0; h < 2; ++h)
-          if (needs(h, begin, end)) issue_qk(h, 0);
-        if (lane == 0) tc::mma_commit(tc::smem_u32(&sm.k_empty[0]));
-        __syncwarp();
-      }
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j % NS, s_next = (j + 1) % NS;
-        const bool more = walk.next(next_begin, next_end);
-        ok = wait_bounded(tc::smem_u32(&sm.v_full[s]), (uint32_t)(j / NS) & 1u, abort_flag, p.err);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        if (end - begin < BKV) {
-          // keys behind the segment: whatever lies there becomes zero before it meets P's zeros
-          const int keys = BKV - (end - begin);
-          for (int c = lane; c < keys * 8 * NB; c += 32) {
-            const int b = c / (keys * 8), rest = c - b * keys * 8;
-            *reinterpret_cast<uint4*>(sm.v[s][b] + (end - begin) * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
-          }
-          tc::fence_proxy_async_smem();
-          __syncwarp();
-        }
-        bool k_ready = false;
-        for (int h = 0; h < 2 && ok; ++h) {
-          if (needs(h, begin, end)) {
-            ok = wait_bounded(tc::smem_u32(&sm.p_full[h]), (uint32_t)sequence[h] & 1u, abort_flag, p.err);
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            tc::fence_after_sync();
-            if (lane == 0) {
-              const uint32_t v_addr = tc::smem_u32(sm.v[s][0]);
-              const uint32_t p_tmem = tmem_base + (uint32_t)(S_COL + h * BKV);
-              const uint32_t d_tmem = tmem_base + (uint32_t)(O_COL + h * D);
+        const uint32_t a = q_lo + (uint32_t)h * (NB * Q_BLOCK >> 4), b = k_lo + (uint32_t)s * (TILE_BYTES >> 4);
 #pragma unroll
-              for (int t = 0; t < BKV / 16; ++t)
-                tc::mma_f16_ts(d_tmem, p_tmem + t * 8, desc_v(v_addr + t * 2048), idesc_pv<D, FP16>(),
-                               (t || sequence[h]) ? 1u : 0u);
-              tc::mma_commit(tc::smem_u32(&sm.o_full[h]));
-            }
-            __syncwarp();
-            ++sequence[h];
-            pending[h] = true;
-          }
-          if (more && needs(h, next_begin, next_end)) {
-            if (!k_ready) ok = wait_bounded(tc::smem_u32(&sm.k_full[s_next]), (uint32_t)((j + 1) / NS) & 1u, abort_flag, p.err);
-            k_ready = true;
-            // the next S takes the place of P: its product has to be done
-            if (ok && pending[h]) {
-              ok = wait_bounded(tc::smem_u32(&sm.o_full[h]), (uint32_t)(sequence[h] - 1) & 1u, abort_flag, p.err);
-              pending[h] = false;
-            }
-            if (!(ok = __all_sync(0xffffffffu, ok))) break;
-            tc::fence_after_sync();
-            issue_qk(h, s_next);
-          }
-        }
-        if (!ok) break;
-        if (more && !k_ready) {  // no half needs the next tile; its stage is released all the same
-          ok = wait_bounded(tc::smem_u32(&sm.k_full[s_next]), (uint32_t)((j + 1) / NS) & 1u, abort_flag, p.err);
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        }
-        if (lane == 0) {
-          tc::mma_commit(tc::smem_u32(&sm.v_empty[s]));
-          if (more) tc::mma_commit(tc::smem_u32(&sm.k_empty[s_next]));
-        }
-        __syncwarp();
-        begin = next_begin, end = next_end;
+        for (int t = 0; t < D / 16; ++t)
+          mma_ss(tmem_base + (uint32_t)s_col(h), a + (uint32_t)(((t >> 2) * Q_BLOCK + (t & 3) * 32) >> 4),
+                 b + (uint32_t)(((t >> 2) * KV_BLOCK + (t & 3) * 32) >> 4), idesc_qk<FP16>(), t > 0);
+        tc::mma_commit(tc::smem_u32(&sm.s_full[h]));
+        ++scores[h];
+      };
+      const auto issue_pv = [&](int h, int s) {
+        const uint32_t buffer = outputs[h] & 1u;
+        await(&sm.p_full[h][buffer], outputs[h] >> 1);
+        if (!ok) return;
+        tc::fence_after_sync();
+        const uint32_t b = v_lo + (uint32_t)s * (TILE_BYTES >> 4);
+#pragma unroll
+        for (int t = 0; t < BKV / 16; ++t)
+          mma_ts(tmem_base + (uint32_t)o_col<D>(h), tmem_base + (uint32_t)p_col(h, 0) + buffer * 32u + t * 8,
+                 b + t * (2048 >> 4), idesc_pv<D, FP16>(), t > 0 || outputs[h] > 0);
+        tc::mma_commit(tc::smem_u32(&sm.o_full[h][buffer]));
+        ++outputs[h];
+      };
+      await(&sm.q_full, 0);
+      await(&sm.k_full[0], 0);
+      walk.next(begin, end);
+      needed[0] = needs(0, begin, end), needed[1] = needs(1, begin, end);
+      if (needed[0]) issue_qk(0, 0);
+      if (needed[1]) issue_qk(1, 0);
+      if (ok) tc::mma_commit(tc::smem_u32(&sm.k_empty[0]));
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        // In this order the halves fall half a tile apart: half 1's next S follows half 0's P.
+        const int s = j % NS, s_next = (j + 1) % NS;
+        const bool more = walk.next(begin, end);
+        next[0] = more && needs(0, begin, end), next[1] = more && needs(1, begin, end);
+        if (more) await(&sm.k_full[s_next], (uint32_t)(j + 1) / NS);
+        if (next[0]) issue_qk(0, s_next);
+        await(&sm.v_clean[s], (uint32_t)j / NS);
+        if (needed[0]) issue_pv(0, s);
+        if (next[1]) issue_qk(1, s_next);
+        if (more && ok) tc::mma_commit(tc::smem_u32(&sm.k_empty[s_next]));
+        if (needed[1]) issue_pv(1, s);
+        if (ok) tc::mma_commit(tc::smem_u32(&sm.v_empty[s]));
+        needed[0] = next[0], needed[1] = next[1];
       }
-      if (lane == 0) {  // every product has ended before tensor memory is freed
-        tc::mma_commit(tc::smem_u32(&sm.drain));
-        const uint64_t start = global_ns();
-        while (!tc::mbar_try_wait(tc::smem_u32(&sm.drain), 0) && global_ns() - start < WAIT_LIMIT_NS) {
-        }
+      // Every product has ended before tensor memory is freed.
+      tc::mma_commit(tc::smem_u32(&sm.drain));
+      const uint64_t start = global_ns();
+      while (!tc::mbar_try_wait(tc::smem_u32(&sm.drain), 0) && global_ns() - start < WAIT_LIMIT_NS) {
       }
-      __syncwarp();
     }
-   }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-    // ------------------------------------------------------------ softmax, one thread per row
-    const int h = warp >> 2;
-    const uint32_t lanes = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t s_tmem = lanes + (uint32_t)(S_COL + h * BKV), o_tmem = lanes + (uint32_t)(O_COL + h * D);
-    const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
-    const float two_over_cap2 = CAP ? 2.f * LOG2E * p.scale / p.cap : 0.f;
-    const float slope2 = BIAS ? __ldg(p.slopes + head) * LOG2E : 0.f;
-    float m = -INFINITY, l = 0.f;
-    int sequence = 0;
-    bool ok = true, redo = false;
+    __syncwarp();
+   } else if (warp == SOFTMAX_WARPS + 2) {
+    // ------------------------------------------------------------ keys behind a segment: whatever
+    // lies there in V becomes zero before it meets P's zeros
     Walk walk(sm.segments, first_tile, last_tile);
     int begin, end;
     for (int j = 0; walk.next(begin, end); ++j) {
-      if (!needs(h, begin, end)) continue;
-      ok = wait_bounded(tc::smem_u32(&sm.s_full[h]), (uint32_t)sequence & 1u, abort_flag, p.err);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      const int s = j % NS;
+      const bool ok = wait_bounded(tc::smem_u32(&sm.v_full[s]), (uint32_t)(j / NS) & 1u, abort_flag, p.err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const int keys = BKV - (end - begin);
+      if (keys > 0) {
+        for (int c = lane; c < keys * 8 * NB; c += 32) {
+          const int b = c / (keys * 8), rest = c - b * keys * 8;
+          *reinterpret_cast<uint4*>(sm.v[s][b] + (end - begin) * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
+        }
+        tc::fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.v_clean[s]));
+    }
+   }
+  } else {
+    // ------------------------------------------------------------ softmax, one thread per row
+    const int h = warp >> 2;
+    const uint32_t lanes = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t s_tmem = lanes + (uint32_t)s_col(h), o_tmem = lanes + (uint32_t)o_col<D>(h);
+    const int hull_lo = sm.hull[h][0], hull_hi = sm.hull[h][1];
+    const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
+    const float factor = CAP ? p.scale / p.cap : 0.f;
+    const float slope2 = BIAS ? __ldg(p.slopes + head) * LOG2E : 0.f;
+    // Keys that every row of the warp sees (rows without keys do not count), and the keys that its rows stand at.
+    const bool has_keys = hi > lo;
+    const int all_lo = __reduce_max_sync(0xffffffffu, has_keys ? lo : 0);
+    const int all_hi = __reduce_min_sync(0xffffffffu, has_keys ? hi : 0x7FFFFFFF);
+    const int first_pos = __reduce_min_sync(0xffffffffu, pos), last_pos = __reduce_max_sync(0xffffffffu, pos);
+    // Reference maximum of the stored exponentials, at most 2^16 below the row's own.
+    float m = -INFINITY;
+    float l = 0.f;
+    int sequence = 0;
+    bool ok = true, redo = false;
+    const auto await = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag, p.err);
+      __syncwarp();
       tc::fence_after_sync();
-      float s[BKV];
+    };
+    Walk walk(sm.segments, first_tile, last_tile);
+    int begin, end;
+    for (int j = 0; walk.next(begin, end); ++j) {
+      if (begin >= hull_hi || end <= hull_lo) continue;
+      const uint32_t buffer = (uint32_t)sequence & 1u;
+      const uint32_t p_tmem = lanes + (uint32_t)p_col(h, 0) + buffer * 32u;
+      await(&sm.s_full[h], sequence);
+      float2 s[BKV / 2];
       {
-        uint32_t raw[4][32];
+        uint32_t raw[2][32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tc::tmem_ld_32x32b_x32(s_tmem + i * 32, raw[i]);
+        for (int i = 0; i < 2; ++i) tc::tmem_ld_32x32b_x32(s_tmem + i * 32, raw[i]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < BKV; ++i) s[i] = __uint_as_float(raw[i >> 5][i & 31]);
+        for (int i = 0; i < BKV / 2; ++i)
+          s[i] = make_float2(__uint_as_float(raw[i >> 4][2 * i & 31]), __uint_as_float(raw[i >> 4][(2 * i & 31) + 1]));
       }
-      if (CAP) {
-#pragma unroll
-        for (int i = 0; i < BKV; ++i) s[i] = capped_log2(s[i], two_over_cap2, cap2);
-      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.s_free[h]));
+      if (CAP) cap_scores(s, factor, cap2);
       if (BIAS) {
-        const float from = (float)(begin - pos);
+        const int from = begin - pos;  // of the tile's first key, from the row's own
+        const float2 unit = both(CAP ? 1.f : scale2);
+        if (begin + BKV <= first_pos || begin >= last_pos) {
+          // the whole tile on one side of the rows: the distance is linear in the key
+          const float slope = here(begin >= last_pos ? -slope2 : slope2), base = slope * (float)from;
 #pragma unroll
-        for (int i = 0; i < BKV; ++i) s[i] = fmaf(-slope2, fabsf(from + (float)i), CAP ? s[i] : s[i] * scale2);
+          for (int i = 0; i < BKV / 2; ++i)
+            s[i] = fma2(s[i], unit, make_float2(fmaf(slope, (float)(2 * i), base), fmaf(slope, (float)(2 * i + 1), base)));
+        } else {
+#pragma unroll
+          for (int i = 0; i < BKV / 2; ++i)
+            s[i] = fma2(s[i], unit, make_float2(-slope2 * fabsf((float)from + (float)(2 * i)),
+                                                -slope2 * fabsf((float)from + (float)(2 * i + 1))));
+        }
       }
-      const int c0 = lo - begin, c1 = min(hi, end) - begin;  // columns that this row sees
-      if (!__all_sync(0xffffffffu, c0 <= 0 && c1 >= BKV)) {
+      if (begin < all_lo || begin + BKV > all_hi) {
+        const int c0 = lo - begin, c1 = min(hi, end) - begin;  // columns that this row sees
 #pragma unroll
-        for (int i = 0; i < BKV; ++i) s[i] = i >= c0 && i < c1 ? s[i] : -INFINITY;
+        for (int i = 0; i < BKV / 2; ++i) {
+          s[i].x = 2 * i >= c0 && 2 * i < c1 ? s[i].x : -INFINITY;
+          s[i].y = 2 * i + 1 >= c0 && 2 * i + 1 < c1 ? s[i].y : -INFINITY;
+        }
         // values that are not finite: exponent bits all ones
         const int st = j % NS;
-        ok = wait_bounded(tc::smem_u32(&sm.v_full[st]), (uint32_t)(j / NS) & 1u, abort_flag, p.err);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        await(&sm.v_full[st], (uint32_t)j / NS);
         constexpr uint32_t EXP = FP16 ? 0x7C00u : 0x7F80u;
         bool found = false;
         for (int c = lane; c < (end - begin) * 8; c += 32) {
@@ -525,68 +650,77 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         redo = redo || __any_sync(0xffffffffu, found);
       }
-      float top[4] = {s[0], s[1], s[2], s[3]};
+      // Exponentials against the reference at hand, which the tiles before have set.  Only where a row
+      // has none yet, or its sum says that it was too low for P's type, is the tile's maximum
+      // taken, O rescaled and the tile done again: a maximum of every tile, which the exponentials
+      // would wait for, is not needed.
+      const float2 unit = both(CAP || BIAS ? 1.f : scale2);
+      if (sequence > 1) await(&sm.o_full[h][buffer], (sequence >> 1) - 1);  // this P's last product has ended
+      for (bool again = false;; again = true) {
+        const float2 offset = both(m == -INFINITY ? 0.f : RAISE<FP16> - m);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int i = 4; i < BKV; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
-      float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-      if (!CAP && !BIAS) m_new *= scale2;
-      const bool rise = m_new > m + RESCALE;
-      if (__any_sync(0xffffffffu, rise)) {
+        for (int part = 0; part < 2; ++part) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 z = CAP || BIAS ? add2(s[part * 16 + i], offset) : fma2(s[part * 16 + i], unit, offset);
+            const float2 e = make_float2(ex2(z.x), ex2(z.y));
+            sum[i & 1] = add2(sum[i & 1], e);
+            packed[i] = pack2<FP16>(e.x, e.y);
+          }
+          tc::tmem_st_32x32b_x16(p_tmem + part * 16, packed);
+        }
+        sum[0] = add2(sum[0], sum[1]);
+        const float total = sum[0].x + sum[0].y;
+        const bool low = has_keys && (m == -INFINITY || !(total <= P_LIMIT));
+        if (again || !__any_sync(0xffffffffu, low)) {
+          l += total;
+          break;
+        }
+        float top[4] = {s[0].x, s[0].y, s[1].x, s[1].y};
+#pragma unroll
+        for (int i = 2; i < BKV / 2; ++i) top[i & 3] = max3(top[i & 3], s[i].x, s[i].y);
+        float m_new = max3(fmaxf(top[0], top[1]), top[2], top[3]);
+        if (!CAP && !BIAS) m_new *= scale2;
         float a = 1.f;
-        if (rise) {
+        if (m_new > m) {
           a = m == -INFINITY ? 0.f : ex2(m - m_new);
           m = m_new;
           l *= a;
         }
         __syncwarp();
-        if (sequence > 0) {
-          ok = wait_bounded(tc::smem_u32(&sm.o_full[h]), (uint32_t)(sequence - 1) & 1u, abort_flag, p.err);
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
-          tc::fence_after_sync();
+        if (sequence > 0) {  // once the product before has ended
+          await(&sm.o_full[h][buffer ^ 1u], (sequence - 1) >> 1);
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t raw[32];
-            tc::tmem_ld_32x32b_x32(o_tmem + i * 32, raw);
+          for (int i = 0; i < D / 16; ++i) {  // sixteen columns at a time: the scores stay in registers
+            uint32_t raw[16];
+            tc::tmem_ld_32x32b_x16(o_tmem + i * 16, raw);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int t = 0; t < 32; ++t) raw[t] = __float_as_uint(__uint_as_float(raw[t]) * a);
-            tc::tmem_st_32x32b_x32(o_tmem + i * 32, raw);
+            for (int t = 0; t < 16; ++t) raw[t] = __float_as_uint(__uint_as_float(raw[t]) * a);
+            tc::tmem_st_32x32b_x16(o_tmem + i * 16, raw);
           }
         }
       }
-      const float ref = m == -INFINITY ? 0.f : m - RAISE<FP16>;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const int at = half * 64 + 2 * i;
-          const float a = ex2(CAP || BIAS ? s[at] - ref : fmaf(s[at], scale2, -ref));
-          const float b = ex2(CAP || BIAS ? s[at + 1] - ref : fmaf(s[at + 1], scale2, -ref));
-          sum[(2 * i) & 3] += a, sum[(2 * i + 1) & 3] += b;
-          packed[i] = pack2<FP16>(a, b);
-        }
-        tc::tmem_st_32x32b_x32(s_tmem + half * 32, packed);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.p_full[h]));
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.p_full[h][buffer]));
       ++sequence;
     }
     // ------------------------------------------------------------ output
     const int r = h * BQ + (warp & 3) * 32 + lane;
     const long long row = row0 + r;
     const bool valid = doc >= 0;
-    if (ok && sequence > 0) ok = wait_bounded(tc::smem_u32(&sm.o_full[h]), (uint32_t)(sequence - 1) & 1u, abort_flag, p.err);
+    if (sequence > 0) await(&sm.o_full[h][(sequence - 1) & 1], (sequence - 1) >> 1);
     if (__all_sync(0xffffffffu, ok)) {
       if (redo) {
         rows_key_by_key<D, FP16>(p, sm.segments, first_tile, last_tile, row0 + r - lane, head, lo, hi, pos, valid, split);
       } else {
         tc::fence_after_sync();
-        const float inv = p.splits == 1 ? inverse_sum(l, hi > lo) : 1.f;
+        if (!has_keys) m = -INFINITY, l = 0.f;
+        const float inv = p.splits == 1 ? inverse_sum(l, has_keys) : 1.f;
         const long long at = (split * p.q_rows + row) * p.heads + head;
         if (valid && p.splits > 1) p.part_ml[at] = make_float2(m, l);
 #pragma unroll
@@ -597,7 +731,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
             tc::tmem_ld_32x32b_x32(o_tmem + i * 32, raw);
             tc::tmem_wait_ld();
           }
-          if (l == 0.f && inv == 0.f) {  // no key: whatever tensor memory holds
+          if (!has_keys) {  // whatever tensor memory holds
 #pragma unroll
             for (int t = 0; t < 32; ++t) raw[t] = 0u;
           }
@@ -636,9 +770,9 @@ int launch(const Params& p, cudaStream_t s) {
   if (grid > 0x7FFFFFFFLL) return fail(MUSC_B200_ERR_INVALID, "masked_attention: too many rows and heads");
   const int qw = p.heads * D, kw = p.kv_heads * D;
   CUtensorMap mq, mk, mv;
-  MUSC_TRY(make_token_map(&mq, p.q, p.q_rows, qw, p.q_rows > 1 ? p.q_stride : qw, FP16));
-  MUSC_TRY(make_token_map(&mk, p.k, p.kv_rows, kw, p.kv_rows > 1 ? p.k_stride : kw, FP16));
-  MUSC_TRY(make_token_map(&mv, p.v, p.kv_rows, kw, p.kv_rows > 1 ? p.v_stride : kw, FP16));
+  MUSC_TRY(make_token_map(&mq, p.q, p.q_rows, qw, p.q_rows > 1 ? p.q_stride : qw, FP16, BQ));
+  MUSC_TRY(make_token_map(&mk, p.k, p.kv_rows, kw, p.kv_rows > 1 ? p.k_stride : kw, FP16, BKV));
+  MUSC_TRY(make_token_map(&mv, p.v, p.kv_rows, kw, p.kv_rows > 1 ? p.v_stride : kw, FP16, BKV));
   const auto kernel = tiles_kernel<D, FP16, CAP, BIAS>;
   MUSC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES<D>));
   kernel<<<(unsigned)grid, THREADS, SMEM_BYTES<D>, s>>>(mq, mk, mv, p);
@@ -655,7 +789,7 @@ int launch_form(const Params& p, cudaStream_t s) {
 
 int tiles_splits(long long units, long long kv_bound) {
   const long long want = 148 / std::max<long long>(units, 1);
-  const long long most = kv_bound / (4 * BKV);  // four tiles at least for each split
+  const long long most = kv_bound / (8 * BKV);  // eight tiles at least for each split
   return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, most), 32));
 }
 
