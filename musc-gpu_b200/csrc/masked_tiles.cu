@@ -9,9 +9,9 @@
 //                   per row: S out of tensor memory, cap, bias, mask, running maximum and
 //                   sum in 32 bits, P rounded to 16 bits back into tensor memory over S;
 //   warp 8          TMA: Q once, K and V tiles through a ring;
-//   warp 9          one thread issues tcgen05.mma: S_h = Q_h K^T (128 x 128 x D, both from
-//                   shared memory) and O_h += P_h V (128 x D x 128, P from tensor memory);
-//   warp 10         zeroes the end of V's tiles that reach past their keys.
+//   warps 9, 10     one thread for each half issues tcgen05.mma: S_h = Q_h K^T (128 x 64 x D,
+//                   both from shared memory) and O_h += P_h V (128 x D x 64, P from tensor memory);
+//   warp 11         zeroes the end of V's tiles that reach past their keys.
 // While one half's softmax runs, the tensor cores work for the other: the exponentials
 // (16 a cycle and SM: 1024 cycles for 128 x 128) bound the kernel for D = 64 (256 cycles of
 // products at the tensor cores' rate) and for D = 128 (512).  O stays in tensor memory and is
@@ -36,7 +36,7 @@ constexpr int ROWS = 2 * BQ;
 constexpr int BKV = 64;    // keys of a tile
 constexpr int Q_BLOCK = BQ * 128, KV_BLOCK = BKV * 128;  // bytes of 64 elements (a swizzle row) of all rows
 constexpr int SOFTMAX_WARPS = 8;
-constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);  // the last warp is idle
+constexpr int THREADS = 32 * (SOFTMAX_WARPS + 4);
 constexpr int TMEM_COLS = 512;
 // Tensor memory: per half S (64 columns), two buffers of P (32 each) and O (D).
 constexpr int s_col(int h) { return h * 64; }
@@ -44,8 +44,7 @@ constexpr int p_col(int h, int buffer) { return 128 + h * 64 + buffer * 32; }
 template <int D> constexpr int o_col(int h) { return 256 + h * D; }
 constexpr float P_LIMIT = 65504.f;  // largest sum of a row's stored exponentials over a tile: each fits fp16
 constexpr int SHARED_DOCS = 1024;  // offsets searched in shared memory up to this many documents
-constexpr uint64_t WAIT_LIMIT_NS = 2000000000ull;
-constexpr uint32_t SLEEP_NS = 1000000;
+constexpr uint32_t WAIT_TRIES = 1u << 20, SLEEP_NS = 2000;
 template <int D> constexpr int STAGES = D == 64 ? 8 : 4;
 
 template <int D>
@@ -54,11 +53,10 @@ struct Smem {
   uint8_t k[STAGES<D>][D / 64][KV_BLOCK];
   uint8_t v[STAGES<D>][D / 64][KV_BLOCK];
   uint64_t q_full;
-  uint64_t k_full[STAGES<D>], k_empty[STAGES<D>];
-  uint64_t v_full[STAGES<D>], v_clean[STAGES<D>], v_empty[STAGES<D>];
+  uint64_t full[STAGES<D>], clean[STAGES<D>], empty[STAGES<D>];
   uint64_t s_full[2], s_free[2];        // per half
   uint64_t p_full[2][2], o_full[2][2];  // per half and buffer of P
-  uint64_t drain;
+  uint64_t drained[2];
   union {
     int offsets[SHARED_DOCS + 1];  // while the rows' documents are looked up
     int2 segments[ROWS];           // then: key ranges [x, y) that the CTA walks
@@ -72,20 +70,24 @@ struct Smem {
 };
 template <int D> constexpr size_t SMEM_BYTES = sizeof(Smem<D>) + 1024;
 
-// Bounded wait.  The thread sleeps in try_wait (a warp that polled instead took up to 40 % of
-// its scheduler from the softmax warps there); the clock is read only after it has slept.
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  if (tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) return true;
-  const uint64_t start = global_ns();
-  while (!tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) {
+// Bounded wait: after WAIT_TRIES tries (each sleeps for up to SLEEP_NS, so at most two
+// seconds in all) the CTA's abort flag is raised, which ends every other wait and is reported
+// when the CTA ends.  Few instructions: the waits stand between the products and exponentials.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (uint32_t tries = 0; tries < WAIT_TRIES; ++tries) {
+    if (tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) return true;
     if (*abort_flag) return false;
-    if (global_ns() - start > WAIT_LIMIT_NS) {
-      *abort_flag = 1;
-      atomicExch(err, MUSC_B200_ERR_TIMEOUT);
-      return false;
-    }
   }
-  return true;
+  *abort_flag = 1;
+  return false;
+}
+
+// Waits for work in flight whether or not the CTA has given up.
+__device__ __forceinline__ void drain(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t tries = 0; tries < WAIT_TRIES; ++tries)
+    if (tc::mbar_try_wait_for(bar, parity, SLEEP_NS)) return;
 }
 
 // Shared-memory matrix descriptors in the 128-byte swizzle, 8-row groups 1024 bytes apart.  The
@@ -321,11 +323,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   if (threadIdx.x == 256) {
     tc::mbar_init(tc::smem_u32(&sm.q_full), 1);
     for (int s = 0; s < NS; ++s) {
-      tc::mbar_init(tc::smem_u32(&sm.k_full[s]), 1);
-      tc::mbar_init(tc::smem_u32(&sm.k_empty[s]), 1);
-      tc::mbar_init(tc::smem_u32(&sm.v_full[s]), 1);
-      tc::mbar_init(tc::smem_u32(&sm.v_clean[s]), 1);
-      tc::mbar_init(tc::smem_u32(&sm.v_empty[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.full[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.clean[s]), 1);
+      tc::mbar_init(tc::smem_u32(&sm.empty[s]), 2);
     }
     for (int h = 0; h < 2; ++h) {
       tc::mbar_init(tc::smem_u32(&sm.s_full[h]), 1);
@@ -334,8 +334,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         tc::mbar_init(tc::smem_u32(&sm.p_full[h][b]), SOFTMAX_WARPS / 2);
         tc::mbar_init(tc::smem_u32(&sm.o_full[h][b]), 1);
       }
+      tc::mbar_init(tc::smem_u32(&sm.drained[h]), 1);
     }
-    tc::mbar_init(tc::smem_u32(&sm.drain), 1);
     sm.abort_flag = 0;
     sm.hull[0][0] = sm.hull[1][0] = 0x7FFFFFFF;
     sm.hull[0][1] = sm.hull[1][1] = 0;
@@ -430,8 +430,6 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   const int first_tile = (int)((long long)sm.n_tiles * split / p.splits);
   const int last_tile = (int)((long long)sm.n_tiles * (split + 1) / p.splits);
   const int n_tiles = last_tile - first_tile;
-  // Whether a half has a row that may see keys [begin, end).
-  const auto needs = [&](int h, int begin, int end) { return begin < sm.hull[h][1] && end > sm.hull[h][0]; };
 
   if (warp >= SOFTMAX_WARPS) {
    if (warp == SOFTMAX_WARPS) {
@@ -443,114 +441,93 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         for (int b = 0; b < NB; ++b)
           tc::tma_load_2d(tc::smem_u32(sm.q[h][b]), &map_q, head * D + b * 64, (int)row0 + h * BQ, qf);
       Walk walk(sm.segments, first_tile, last_tile);
-      int begin, end, j = 0;
-      int k_issued = 0, v_issued = 0;
-      for (; walk.next(begin, end); ++j) {
-        const int s = j % NS;
-        const uint32_t ph = (uint32_t)(j / NS) & 1u;
-        if (!wait_bounded(tc::smem_u32(&sm.k_empty[s]), ph ^ 1u, abort_flag, p.err)) break;
-        const uint32_t kf = tc::smem_u32(&sm.k_full[s]);
-        tc::mbar_arrive_expect_tx(kf, TILE_BYTES);
-        for (int b = 0; b < NB; ++b) tc::tma_load_2d(tc::smem_u32(sm.k[s][b]), &map_k, kv_head * D + b * 64, begin, kf);
-        k_issued = j + 1;
-        if (!wait_bounded(tc::smem_u32(&sm.v_empty[s]), ph ^ 1u, abort_flag, p.err)) break;
-        const uint32_t vf = tc::smem_u32(&sm.v_full[s]);
-        tc::mbar_arrive_expect_tx(vf, TILE_BYTES);
-        for (int b = 0; b < NB; ++b) tc::tma_load_2d(tc::smem_u32(sm.v[s][b]), &map_v, kv_head * D + b * 64, begin, vf);
-        v_issued = j + 1;
+      int begin, end, issued = 0;
+      while (walk.next(begin, end)) {
+        const int s = issued % NS;
+        if (!wait_bounded(tc::smem_u32(&sm.empty[s]), ((uint32_t)(issued / NS) & 1u) ^ 1u, abort_flag)) break;
+        const uint32_t full = tc::smem_u32(&sm.full[s]);
+        tc::mbar_arrive_expect_tx(full, 2 * TILE_BYTES);
+        for (int b = 0; b < NB; ++b) {
+          tc::tma_load_2d(tc::smem_u32(sm.k[s][b]), &map_k, kv_head * D + b * 64, begin, full);
+          tc::tma_load_2d(tc::smem_u32(sm.v[s][b]), &map_v, kv_head * D + b * 64, begin, full);
+        }
+        ++issued;
       }
       // Let every copy this thread issued land before the CTA can exit.
-      const uint64_t start = global_ns();
-      while (!tc::mbar_try_wait(qf, 0) && global_ns() - start < WAIT_LIMIT_NS) {
-      }
-      for (int i = 0; i < NS; ++i) {
-        for (int which = 0; which < 2; ++which) {
-          const int t = (which ? v_issued : k_issued) - 1 - i;
-          if (t < 0) continue;
-          const uint32_t bar = tc::smem_u32(which ? &sm.v_full[t % NS] : &sm.k_full[t % NS]);
-          const uint64_t t0 = global_ns();
-          while (!tc::mbar_try_wait(bar, (uint32_t)(t / NS) & 1u) && global_ns() - t0 < WAIT_LIMIT_NS) {
-          }
-        }
-      }
+      drain(qf, 0);
+      for (int t = max(issued - NS, 0); t < issued; ++t) drain(tc::smem_u32(&sm.full[t % NS]), (uint32_t)(t / NS) & 1u);
     }
-   } else if (warp == SOFTMAX_WARPS + 1) {
-    // ------------------------------------------------------------ MMA issuer: one thread, and
-    // little code, since the softmax warps' loops keep it out of the instruction caches
+   } else if (warp <= SOFTMAX_WARPS + 2) {
+    // ------------------------------------------------------------ MMA issuers, one thread for each
+    // half.  A wait takes a place in the scheduler's queue behind up to 32 exponentials of the
+    // softmax warps there, some 270 cycles even if the barrier is ready, so one thread could
+    // not keep up with both halves, and each waits for as little as it can.
     if (n_tiles > 0 && tc::elect_one()) {
+      const int h = warp - SOFTMAX_WARPS - 1;
+      const int hull_lo = sm.hull[h][0], hull_hi = sm.hull[h][1];
       Walk walk(sm.segments, first_tile, last_tile);
-      int begin = 0, end = 0;
-      // Products of each half so far (S and P V), and whether the half needs this tile and the next.
-      uint32_t scores[2] = {0, 0}, outputs[2] = {0, 0};
-      bool ok = true, needed[2], next[2];
-      const uint32_t q_lo = desc_lo_k(tc::smem_u32(sm.q)), k_lo = desc_lo_k(tc::smem_u32(sm.k));
+      uint32_t scores = 0, outputs = 0;  // S and P V products so far
+      bool ok = true;
+      const uint32_t q_lo = desc_lo_k(tc::smem_u32(sm.q[h])), k_lo = desc_lo_k(tc::smem_u32(sm.k));
       const uint32_t v_lo = desc_lo_v(tc::smem_u32(sm.v));
+      const uint32_t s_tmem = tmem_base + (uint32_t)s_col(h), o_tmem = tmem_base + (uint32_t)o_col<D>(h);
       const auto await = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag, p.err);
+        ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag);
       };
-      // S of half h for the tile in stage s, once the softmax has read the S before.
-      const auto issue_qk = [&](int h, int s) {
-        if (scores[h] > 0) await(&sm.s_free[h], scores[h] - 1);
+      int waiting = -1;  // stage of the tile whose second product has not been issued
+      const auto issue_pv = [&]() {
+        const uint32_t buffer = outputs & 1u;
+        await(&sm.p_full[h][buffer], outputs >> 1);
         if (!ok) return;
         tc::fence_after_sync();
-        const uint32_t a = q_lo + (uint32_t)h * (NB * Q_BLOCK >> 4), b = k_lo + (uint32_t)s * (TILE_BYTES >> 4);
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-          mma_ss(tmem_base + (uint32_t)s_col(h), a + (uint32_t)(((t >> 2) * Q_BLOCK + (t & 3) * 32) >> 4),
-                 b + (uint32_t)(((t >> 2) * KV_BLOCK + (t & 3) * 32) >> 4), idesc_qk<FP16>(), t > 0);
-        tc::mma_commit(tc::smem_u32(&sm.s_full[h]));
-        ++scores[h];
-      };
-      const auto issue_pv = [&](int h, int s) {
-        const uint32_t buffer = outputs[h] & 1u;
-        await(&sm.p_full[h][buffer], outputs[h] >> 1);
-        if (!ok) return;
-        tc::fence_after_sync();
-        const uint32_t b = v_lo + (uint32_t)s * (TILE_BYTES >> 4);
+        const uint32_t b = v_lo + (uint32_t)waiting * (TILE_BYTES >> 4);
 #pragma unroll
         for (int t = 0; t < BKV / 16; ++t)
-          mma_ts(tmem_base + (uint32_t)o_col<D>(h), tmem_base + (uint32_t)p_col(h, 0) + buffer * 32u + t * 8,
-                 b + t * (2048 >> 4), idesc_pv<D, FP16>(), t > 0 || outputs[h] > 0);
+          mma_ts(o_tmem, tmem_base + (uint32_t)p_col(h, 0) + buffer * 32u + t * 8, b + t * (2048 >> 4), idesc_pv<D, FP16>(),
+                 t > 0 || outputs > 0);
         tc::mma_commit(tc::smem_u32(&sm.o_full[h][buffer]));
-        ++outputs[h];
+        tc::mma_commit(tc::smem_u32(&sm.empty[waiting]));
+        ++outputs;
+        waiting = -1;
       };
       await(&sm.q_full, 0);
-      await(&sm.k_full[0], 0);
-      walk.next(begin, end);
-      needed[0] = needs(0, begin, end), needed[1] = needs(1, begin, end);
-      if (needed[0]) issue_qk(0, 0);
-      if (needed[1]) issue_qk(1, 0);
-      if (ok) tc::mma_commit(tc::smem_u32(&sm.k_empty[0]));
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        // In this order the halves fall half a tile apart: half 1's next S follows half 0's P.
-        const int s = j % NS, s_next = (j + 1) % NS;
-        const bool more = walk.next(begin, end);
-        next[0] = more && needs(0, begin, end), next[1] = more && needs(1, begin, end);
-        if (more) await(&sm.k_full[s_next], (uint32_t)(j + 1) / NS);
-        if (next[0]) issue_qk(0, s_next);
-        await(&sm.v_clean[s], (uint32_t)j / NS);
-        if (needed[0]) issue_pv(0, s);
-        if (next[1]) issue_qk(1, s_next);
-        if (more && ok) tc::mma_commit(tc::smem_u32(&sm.k_empty[s_next]));
-        if (needed[1]) issue_pv(1, s);
-        if (ok) tc::mma_commit(tc::smem_u32(&sm.v_empty[s]));
-        needed[0] = next[0], needed[1] = next[1];
+      int begin, end;
+#pragma unroll 1
+      for (int j = 0; walk.next(begin, end) && ok; ++j) {
+        const int s = j % NS;
+        await(&sm.clean[s], (uint32_t)j / NS);
+        if (begin >= hull_hi || end <= hull_lo) {  // not this half's
+          if (waiting >= 0) issue_pv();
+          if (ok) tc::mbar_arrive(tc::smem_u32(&sm.empty[s]));
+          continue;
+        }
+        if (scores > 0) await(&sm.s_free[h], scores - 1);  // the softmax has read the S before
+        if (!ok) break;
+        tc::fence_after_sync();
+        const uint32_t b = k_lo + (uint32_t)s * (TILE_BYTES >> 4);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          mma_ss(s_tmem, q_lo + (uint32_t)(((t >> 2) * Q_BLOCK + (t & 3) * 32) >> 4),
+                 b + (uint32_t)(((t >> 2) * KV_BLOCK + (t & 3) * 32) >> 4), idesc_qk<FP16>(), t > 0);
+        tc::mma_commit(tc::smem_u32(&sm.s_full[h]));  // also the end of the P V products issued before
+        ++scores;
+        if (waiting >= 0) issue_pv();
+        waiting = s;
       }
+      if (waiting >= 0) issue_pv();
       // Every product has ended before tensor memory is freed.
-      tc::mma_commit(tc::smem_u32(&sm.drain));
-      const uint64_t start = global_ns();
-      while (!tc::mbar_try_wait(tc::smem_u32(&sm.drain), 0) && global_ns() - start < WAIT_LIMIT_NS) {
-      }
+      tc::mma_commit(tc::smem_u32(&sm.drained[h]));
+      drain(tc::smem_u32(&sm.drained[h]), 0);
     }
     __syncwarp();
-   } else if (warp == SOFTMAX_WARPS + 2) {
+   } else {
     // ------------------------------------------------------------ keys behind a segment: whatever
     // lies there in V becomes zero before it meets P's zeros
     Walk walk(sm.segments, first_tile, last_tile);
     int begin, end;
     for (int j = 0; walk.next(begin, end); ++j) {
       const int s = j % NS;
-      const bool ok = wait_bounded(tc::smem_u32(&sm.v_full[s]), (uint32_t)(j / NS) & 1u, abort_flag, p.err);
+      const bool ok = wait_bounded(tc::smem_u32(&sm.full[s]), (uint32_t)(j / NS) & 1u, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) break;
       const int keys = BKV - (end - begin);
       if (keys > 0) {
@@ -561,7 +538,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         tc::fence_proxy_async_smem();
       }
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.v_clean[s]));
+      if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.clean[s]));
     }
    }
   } else {
@@ -584,7 +561,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     int sequence = 0;
     bool ok = true, redo = false;
     const auto await = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag, p.err);
+      ok = ok && wait_bounded(tc::smem_u32(bar), parity & 1u, abort_flag);
       __syncwarp();
       tc::fence_after_sync();
     };
@@ -634,7 +611,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         // values that are not finite: exponent bits all ones
         const int st = j % NS;
-        await(&sm.v_full[st], (uint32_t)j / NS);
+        await(&sm.full[st], (uint32_t)j / NS);
         constexpr uint32_t EXP = FP16 ? 0x7C00u : 0x7F80u;
         bool found = false;
         for (int c = lane; c < (end - begin) * 8; c += 32) {
@@ -655,7 +632,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
       // taken, O rescaled and the tile done again: a maximum of every tile, which the exponentials
       // would wait for, is not needed.
       const float2 unit = both(CAP || BIAS ? 1.f : scale2);
-      if (sequence > 1) await(&sm.o_full[h][buffer], (sequence >> 1) - 1);  // this P's last product has ended
+      // This P's product of two tiles ago has ended: its thread issued it before this S.
       for (bool again = false;; again = true) {
         const float2 offset = both(m == -INFINITY ? 0.f : RAISE<FP16> - m);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -761,6 +738,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   if (warp == SOFTMAX_WARPS + 1) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem_base, TMEM_COLS);
+    if (lane == 0 && *abort_flag) atomicExch(p.err, MUSC_B200_ERR_TIMEOUT);
   }
 }
 
