@@ -11,16 +11,16 @@
 //   warp 8          TMA: Q once, K and V tiles through a ring;
 //   warps 9, 10     one thread for each half issues tcgen05.mma: S_h = Q_h K^T (128 x 64 x D,
 //                   both from shared memory) and O_h += P_h V (128 x D x 64, P from tensor memory);
-//   warp 11         zeroes the end of V's tiles that reach past their keys.
+//   warp 11         zeroes the end of V's tiles that reach past their keys, and searches V.
 // While one half's softmax runs, the tensor cores work for the other: the exponentials
 // (16 a cycle and SM: 1024 cycles for 128 x 128) bound the kernel for D = 64 (256 cycles of
 // products at the tensor cores' rate) and for D = 128 (512).  O stays in tensor memory and is
 // rescaled only when a row's maximum has risen by more than 2^8 over the one in use.
 //
 // A masked probability is zero, but zero times a NaN or infinite value is NaN.  Keys that no
-// row of the CTA sees (behind a document's last key) are zeroed in V's tile.  In tiles that a
-// warp's rows see only in part the warp looks for such values in V, and where there is one
-// recomputes its rows key by key at the end, skipping what they do not see: rare, slow, right.
+// row of the CTA sees (behind a document's last key) are zeroed in V's tile.  Tiles that some row
+// may not see in whole are searched for such values, and a warp whose rows see such a tile in part
+// recomputes them key by key at the end, skipping what they do not see: rare, slow, right.
 #include "masked.cuh"
 #include "tc.cuh"
 
@@ -64,6 +64,8 @@ struct Smem {
   int lo[ROWS], hi[ROWS], doc[ROWS];
   uint32_t starts[ROWS / 32];      // rows that begin another document than the row before
   int hull[2][2];                  // per half: first key and end of all its rows' keys
+  int common[2];                   // the keys that all rows with keys see: from, to
+  int odd[STAGES<D>];              // V's tile in a stage holds values that are not finite
   int n_segments, n_tiles;
   uint32_t tmem_base;
   int abort_flag;
@@ -339,6 +341,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     sm.abort_flag = 0;
     sm.hull[0][0] = sm.hull[1][0] = 0x7FFFFFFF;
     sm.hull[0][1] = sm.hull[1][1] = 0;
+    sm.common[0] = 0, sm.common[1] = 0x7FFFFFFF;
     tc::fence_barrier_init();
     tc::prefetch_tensormap(&map_q);
     tc::prefetch_tensormap(&map_k);
@@ -377,9 +380,13 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     sm.lo[threadIdx.x] = lo, sm.hi[threadIdx.x] = hi, sm.doc[threadIdx.x] = doc;
     const int first = __reduce_min_sync(0xffffffffu, hi > lo ? lo : 0x7FFFFFFF);
     const int end = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
+    const int all_from = __reduce_max_sync(0xffffffffu, hi > lo ? lo : 0);
+    const int all_to = __reduce_min_sync(0xffffffffu, hi > lo ? hi : 0x7FFFFFFF);
     if (lane == 0) {
       atomicMin(&sm.hull[warp >> 2][0], first);
       atomicMax(&sm.hull[warp >> 2][1], end);
+      atomicMax(&sm.common[0], all_from);
+      atomicMin(&sm.common[1], all_to);
     }
   }
   __syncthreads();
@@ -523,6 +530,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
    } else {
     // ------------------------------------------------------------ keys behind a segment: whatever
     // lies there in V becomes zero before it meets P's zeros
+    const int common_from = sm.common[0], common_to = sm.common[1];
     Walk walk(sm.segments, first_tile, last_tile);
     int begin, end;
     for (int j = 0; walk.next(begin, end); ++j) {
@@ -536,6 +544,21 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
           *reinterpret_cast<uint4*>(sm.v[s][b] + (end - begin) * 128 + rest * 16) = make_uint4(0, 0, 0, 0);
         }
         tc::fence_proxy_async_smem();
+      }
+      if (begin < common_from || begin + BKV > common_to) {
+        // Values that are not finite, in keys that some row may not see: all exponent bits set, so that
+        // one more unit of the exponent carries into the sign, two values of a word at once.
+        constexpr uint32_t EXP = FP16 ? 0x7C007C00u : 0x7F807F80u, UNIT = FP16 ? 0x04000400u : 0x00800080u;
+        uint32_t carry = 0;
+        for (int c = lane; c < (end - begin) * 8; c += 32) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const uint4 w = *reinterpret_cast<const uint4*>(sm.v[s][b] + c * 16);
+            carry |= ((w.x & EXP) + UNIT) | ((w.y & EXP) + UNIT) | ((w.z & EXP) + UNIT) | ((w.w & EXP) + UNIT);
+          }
+        }
+        carry = __reduce_or_sync(0xffffffffu, carry & 0x80008000u);
+        if (lane == 0) sm.odd[s] = carry != 0;
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(tc::smem_u32(&sm.clean[s]));
@@ -602,6 +625,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
                                                 -slope2 * fabsf((float)from + (float)(2 * i + 1))));
         }
       }
+      bool visible = has_keys;
       if (begin < all_lo || begin + BKV > all_hi) {
         const int c0 = lo - begin, c1 = min(hi, end) - begin;  // columns that this row sees
 #pragma unroll
@@ -609,23 +633,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
           s[i].x = 2 * i >= c0 && 2 * i < c1 ? s[i].x : -INFINITY;
           s[i].y = 2 * i + 1 >= c0 && 2 * i + 1 < c1 ? s[i].y : -INFINITY;
         }
-        // values that are not finite: exponent bits all ones
-        const int st = j % NS;
-        await(&sm.full[st], (uint32_t)j / NS);
-        constexpr uint32_t EXP = FP16 ? 0x7C00u : 0x7F80u;
-        bool found = false;
-        for (int c = lane; c < (end - begin) * 8; c += 32) {
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sm.v[st][b] + c * 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t x = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
-              found = found || (x & EXP) == EXP || (x & (EXP << 16)) == (EXP << 16);
-            }
-          }
-        }
-        redo = redo || __any_sync(0xffffffffu, found);
+        visible = c1 > max(c0, 0);
+        await(&sm.clean[j % NS], (uint32_t)j / NS);
+        redo = redo || sm.odd[j % NS] != 0;
       }
       // Exponentials against the reference at hand, which the tiles before have set.  Only where a row
       // has none yet, or its sum says that it was too low for P's type, is the tile's maximum
@@ -650,7 +660,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         sum[0] = add2(sum[0], sum[1]);
         const float total = sum[0].x + sum[0].y;
-        const bool low = has_keys && (m == -INFINITY || !(total <= P_LIMIT));
+        const bool low = visible && (m == -INFINITY || !(total <= P_LIMIT));
         if (again || !__any_sync(0xffffffffu, low)) {
           l += total;
           break;
