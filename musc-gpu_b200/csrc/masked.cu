@@ -9,33 +9,47 @@ namespace masked {
 namespace {
 
 // Joins the splits: out = sum_s w_s O_s / sum_s w_s l_s with w_s = 2^(m_s - max m).  One
-// warp per (row, head); the partial outputs were just written and come out of L2.
+// warp per (row, head); the lanes hold the splits' weights, and the partial outputs, which were
+// just written and come out of L2, are loaded eight splits ahead.
 template <int D, bool FP16>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= p.q_rows * p.heads) return;
-  const long long row = unit / p.heads;
-  const int head = (int)(unit - row * p.heads), lane = threadIdx.x & 31;
-  const int doc = find_document(p, row);
-  if (doc < 0) return;
-  const Interval iv = row_interval(p, doc, row);
+  const int lane = threadIdx.x & 31;
   const long long per_split = p.q_rows * p.heads;
-  float common = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) common = fmaxf(common, p.part_ml[s * per_split + unit].x);
-  common = warp_max(common);
-  float acc[D / 32], total = 0.f;
+  float m[2], l[2], w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {  // splits lane and lane + 32
+    const int s = lane + 32 * i;
+    const float2 ml = s < p.splits ? p.part_ml[s * per_split + unit] : make_float2(-INFINITY, 0.f);
+    m[i] = ml.x, l[i] = ml.y;
+  }
+  if (__any_sync(0xffffffffu, l[0] == NOT_MINE)) return;
+  const float common = warp_max(fmaxf(m[0], m[1]));
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = split_weight(m[i], common);
+    total = fmaf(w[i], l[i], total);
+    if (l[i] == 0.f) w[i] = 0.f;  // nothing was written for it
+  }
+  total = warp_sum(total);
+  float acc[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  const float* part = p.part + unit * D + lane * (D / 32);
+#pragma unroll 8
   for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.part_ml[s * per_split + unit];
-    const float w = split_weight(ml.x, common);
-    total = fmaf(w, ml.y, total);
-    if (w == 0.f && ml.y == 0.f) continue;  // nothing was written for it
-    const float* o = p.part + (s * per_split + unit) * D + lane * (D / 32);
+    const float weight = __shfl_sync(0xffffffffu, s < 32 ? w[0] : w[1], s & 31);
+    float o[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, o[i], acc[i]);
+    for (int i = 0; i < D / 32; ++i) o[i] = weight != 0.f ? part[s * per_split * D + i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(weight, o[i], acc[i]);
   }
-  const float inv = inverse_sum(total, iv.hi > iv.lo);
+  const float inv = inverse_sum(total, common != -INFINITY);
+  const long long row = unit / p.heads;
+  const int head = (int)(unit - row * p.heads);
   uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.out_stride + (long long)head * D + lane * (D / 32);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
@@ -63,8 +77,10 @@ struct Plan {
   size_t ml_offset = 0, bytes = 0;
 };
 
-// Keys that one document can have, as far as the host knows.
-long long kv_bound(const musc_b200_masked_attention_args& a) { return a.q_offsets ? a.kv_rows : a.kv_len; }
+// Keys of a document, as far as the host knows: of packed ones the mean.
+long long mean_keys(const musc_b200_masked_attention_args& a) {
+  return a.q_offsets ? (a.kv_rows + a.documents - 1) / a.documents : a.kv_len;
+}
 
 Plan make_plan(const musc_b200_masked_attention_args& a) {
   Plan plan;
@@ -74,10 +90,10 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   // heads of a key head (up to 16), reading its keys again for every row.
   plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
   if (plan.tiles)
-    plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, kv_bound(a));
+    plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a));
   else
-    plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), kv_bound(a));
-  if (plan.splits > 1) {
+    plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), mean_keys(a), a.q_rows <= a.documents);
+  if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {
     plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;
     plan.bytes = plan.ml_offset + (size_t)plan.splits * rows * sizeof(float2);
   }
@@ -179,6 +195,6 @@ extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args*
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool fp16 = a.dtype == MUSC_B200_F16;
   MUSC_TRY(plan.tiles ? tiles_launch(p, a.head_dim, fp16, s) : rows_launch(p, a.head_dim, fp16, s));
-  if (plan.splits > 1) MUSC_TRY(combine_launch(p, a.head_dim, fp16, s));
+  if (plan.bytes > 0) MUSC_TRY(combine_launch(p, a.head_dim, fp16, s));
   return MUSC_B200_OK;
 }

@@ -13,6 +13,8 @@
 
 #include "common.cuh"
 
+#include <float.h>
+
 namespace musc {
 namespace masked {
 
@@ -60,6 +62,18 @@ __device__ __forceinline__ int find_document(const Params& p, long long row) {
     else hi = mid;
   }
   return lo;
+}
+
+// The same by a converged warp, in one load's time for up to 1024 documents: the lanes count the
+// documents that begin at or before the row.
+__device__ __forceinline__ int find_document_warp(const Params& p, long long row) {
+  if (!p.q_offsets || p.documents > 1024) return find_document(p, row);
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+#pragma unroll 8
+  for (int i = lane; i <= p.documents; i += 32) before += __ldg(p.q_offsets + i) <= row ? 1 : 0;
+  before = __reduce_add_sync(0xffffffffu, before);
+  return before > 0 && before <= p.documents ? before - 1 : -1;
 }
 
 __device__ __forceinline__ Interval row_interval(const Params& p, int doc, long long row) {
@@ -116,6 +130,14 @@ __device__ __forceinline__ float capped_log2(float x, float two_over_cap2, float
 template <bool FP16>
 constexpr float RAISE = FP16 ? 6.f : 0.f;
 
+// A split's partial result of a row and head: its reference maximum and its sum.  The maximum of a
+// row that sees keys is finite even where it met none of them; (-inf, 0) says that it sees no key,
+// (-inf, -1) that it belongs to no document and is not written.
+__device__ __forceinline__ float2 partial_ml(float m, float l, bool any_key) {
+  return make_float2(any_key ? fmaxf(m, -FLT_MAX) : -INFINITY, l);
+}
+constexpr float NOT_MINE = -1.f;
+
 // Weight of a split's partial sums against the row's common maximum.
 __device__ __forceinline__ float split_weight(float m, float common) {
   return m == -INFINITY ? 0.f : ex2(m - common);
@@ -128,11 +150,13 @@ __device__ __forceinline__ float inverse_sum(float l, bool any_key) {
   return 1.f / l;
 }
 
-// Splits of the keys that give `units` CTAs of work enough CTAs (launchers of both kernels).
+// The kernels' launchers, and the splits of the keys that give `units` CTAs of work enough CTAs
+// when a document has about `keys` keys.
+constexpr int MAX_CLUSTER = 8;  // up to so many splits the row kernel joins by itself, without a workspace
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
-int rows_splits(long long units, long long kv_bound);
+int rows_splits(long long units, long long keys, bool single);  // single: one row for each document
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
-int tiles_splits(long long units, long long kv_bound);
+int tiles_splits(long long units, long long keys);
 int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 
 }  // namespace masked

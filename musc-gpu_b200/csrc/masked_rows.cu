@@ -9,8 +9,10 @@
 // ring of its own that cp.async fills STAGES runs ahead, so no barrier stands between a
 // warp's loads and their use; keys past the row's interval are filled with zeros by the copy
 // itself (a masked value that is NaN never reaches a product).  The warps' and the splits'
-// sums are joined at the end by their maxima.
+// sums are joined at the end by their maxima: up to eight splits form a cluster and read each
+// other's sums from shared memory (one launch, no workspace), more leave theirs to combine_kernel.
 #include "masked.cuh"
+#include "tc.cuh"
 
 #include <algorithm>
 
@@ -21,9 +23,14 @@ namespace {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int KEYS = 16;    // keys of a warp's step
-constexpr int STAGES = 4;   // steps in flight per warp: WARPS x STAGES x 64 D bytes a CTA
+constexpr int STAGES = 2;   // steps in flight per warp: WARPS x STAGES x 64 D bytes a CTA
 constexpr int HEADS = 16;   // query heads of a CTA
-constexpr int TARGET_CTAS = 148 * 3;  // CTAs that fill a B200 (148 SMs)
+// Splits.  Three waves of what is resident (148 SMs x 3 CTAs) even out documents of differing lengths:
+// 32 tokens over 8192 keys in 116 us, 132 with one wave.  Where several rows of a document read its keys
+// from L2, one wave keeps them together: 2 rows over 6390 keys in 32 us, 38 with three.
+constexpr int TARGET_SINGLE = 1332, TARGET_SEVERAL = 444;
+constexpr int MIN_KEYS = 256;       // of a split: 465 keys in one take 15 us, in two 21
+constexpr int CLUSTER_KEYS = 4096;  // more keys per split than this, and more than a cluster's splits are taken
 constexpr float RESCALE = 8.f;  // log2 by which a running maximum may lag behind before sums are rescaled
 
 template <int D>
@@ -33,7 +40,18 @@ struct Smem {
     float o[WARPS][HEADS][D + 4];
   };
   float ml[WARPS][HEADS][2];
+  float sums[HEADS][D];        // of the CTA, for its cluster
+  float2 sums_ml[HEADS];
 };
+
+__device__ __forceinline__ uint32_t cluster_address(const void* p, uint32_t rank) {
+  return tc::mapa(tc::smem_u32(p), rank);
+}
+__device__ __forceinline__ float2 load_cluster2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
@@ -73,29 +91,39 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
-template <int D, bool FP16>
+// Eight finished dimensions of a head.
+template <bool FP16>
+__device__ __forceinline__ void store_eight(const Params& p, long long row, int column, const float (&acc)[8], float inv) {
+  uint4 packed;
+  packed.x = pack2<FP16>(acc[0] * inv, acc[1] * inv), packed.y = pack2<FP16>(acc[2] * inv, acc[3] * inv);
+  packed.z = pack2<FP16>(acc[4] * inv, acc[5] * inv), packed.w = pack2<FP16>(acc[6] * inv, acc[7] * inv);
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.out_stride + column) = packed;
+}
+
+template <int D, bool FP16, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
   constexpr int CHUNKS = D / 8;  // 16-byte chunks of a key
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int blocks = (p.group + HEADS - 1) / HEADS;  // CTAs of a key head's group
   // Neighbouring CTAs take neighbouring rows: those of one document share its keys in L2.
-  long long unit = blockIdx.x;
+  long long unit = blockIdx.x / p.splits;
+  const int split = (int)(blockIdx.x - unit * p.splits);
   const long long row = unit % p.q_rows;
   unit /= p.q_rows;
-  const int kv_head = (int)(unit % p.kv_heads);
-  unit /= p.kv_heads;
-  const int block = (int)(unit % blocks), split = (int)(unit / blocks);
-  const int doc = find_document(p, row);
-  if (doc < 0) return;  // uniform over the CTA
+  const int kv_head = (int)(unit % p.kv_heads), block = (int)(unit / p.kv_heads);
+  const int head0 = kv_head * p.group + block * HEADS;
+  const int n_heads = min(HEADS, p.group - block * HEADS);
+  const int doc = find_document_warp(p, row);
+  if (doc < 0) {  // uniform over the CTA and its cluster
+    if (!CLUSTER && p.splits > 1 && threadIdx.x < n_heads)
+      p.part_ml[(split * p.q_rows + row) * p.heads + head0 + threadIdx.x] = make_float2(-INFINITY, NOT_MINE);
+    return;
+  }
   const Interval iv = row_interval(p, doc, row);
   // This split's share of the interval, in whole steps.
   const long long steps = (iv.hi - iv.lo + KEYS - 1) / KEYS;
   const long long first = steps * split / p.splits, last = steps * (split + 1) / p.splits;
-  const int head0 = kv_head * p.group + block * HEADS;
-  const int n_heads = min(HEADS, p.group - block * HEADS);
-
   const uint16_t* k_base = static_cast<const uint16_t*>(p.k) + kv_head * D;
   const uint16_t* v_base = static_cast<const uint16_t*>(p.v) + kv_head * D;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sm.ring[warp][0][0][0]));
@@ -251,39 +279,87 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, sm.o[w][r][d + i], acc[i]);
     }
-    const int head = head0 + r;
-    if (p.splits == 1) {
-      const float inv = inverse_sum(total, iv.hi > iv.lo);
-      uint4 packed;
-      packed.x = pack2<FP16>(acc[0] * inv, acc[1] * inv), packed.y = pack2<FP16>(acc[2] * inv, acc[3] * inv);
-      packed.z = pack2<FP16>(acc[4] * inv, acc[5] * inv), packed.w = pack2<FP16>(acc[6] * inv, acc[7] * inv);
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.out_stride + (long long)head * D + d) = packed;
+    if (CLUSTER) {
+      if (d == 0) sm.sums_ml[r] = partial_ml(common, total, iv.hi > iv.lo);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sm.sums[r][d + i] = acc[i];
+    } else if (p.splits == 1) {
+      store_eight<FP16>(p, row, (head0 + r) * D + d, acc, inverse_sum(total, iv.hi > iv.lo));
     } else {
-      const long long at = (split * p.q_rows + row) * p.heads + head;
-      if (d == 0) p.part_ml[at] = make_float2(common, total);
-      if (common != -INFINITY || total != 0.f) {
+      const long long at = (split * p.q_rows + row) * p.heads + head0 + r;
+      if (d == 0) p.part_ml[at] = partial_ml(common, total, iv.hi > iv.lo);
+      if (total != 0.f) {
         *reinterpret_cast<float4*>(p.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         *reinterpret_cast<float4*>(p.part + at * D + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
       }
     }
   }
+  if (CLUSTER) {
+    // Every CTA of the cluster joins its share of the heads' dimensions, eight at a time.
+    tc::cluster_sync();
+    for (int e = split * THREADS + threadIdx.x; e < n_heads * (D / 8); e += p.splits * THREADS) {
+      const int r = e / (D / 8), d = e % (D / 8) * 8;
+      float2 ml[MAX_CLUSTER];
+      float common = -INFINITY, total = 0.f, acc[8];
+#pragma unroll
+      for (int c = 0; c < MAX_CLUSTER; ++c) {
+        ml[c] = c < p.splits ? load_cluster2(cluster_address(&sm.sums_ml[r], c)) : make_float2(-INFINITY, 0.f);
+        common = fmaxf(common, ml[c].x);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < MAX_CLUSTER; ++c) {
+        const float f = split_weight(ml[c].x, common);
+        total = fmaf(f, ml[c].y, total);
+        if (c >= p.splits || ml[c].y == 0.f) continue;
+        const uint32_t from = cluster_address(&sm.sums[r][d], c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 o = load_cluster2(from + i * 8);
+          acc[2 * i] = fmaf(f, o.x, acc[2 * i]), acc[2 * i + 1] = fmaf(f, o.y, acc[2 * i + 1]);
+        }
+      }
+      store_eight<FP16>(p, row, (head0 + r) * D + d, acc, inverse_sum(total, common != -INFINITY));
+    }
+    tc::cluster_sync();  // no CTA leaves while another reads its sums
+  }
+}
+
+template <int D, bool FP16, bool CLUSTER>
+int launch_as(const Params& p, long long grid, cudaStream_t s) {
+  const auto kernel = rows_kernel<D, FP16, CLUSTER>;
+  MUSC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>)));
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid);
+  config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = sizeof(Smem<D>);
+  config.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CLUSTER ? p.splits : 1;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = CLUSTER ? 1 : 0;
+  MUSC_CUDA(cudaLaunchKernelEx(&config, kernel, p));
+  return MUSC_B200_OK;
 }
 
 template <int D, bool FP16>
 int launch(const Params& p, cudaStream_t s) {
   const long long grid = p.q_rows * p.kv_heads * ((p.group + HEADS - 1) / HEADS) * p.splits;
   if (grid > 0x7FFFFFFFLL) return fail(MUSC_B200_ERR_INVALID, "masked_attention: too many rows and heads");
-  MUSC_CUDA(cudaFuncSetAttribute(rows_kernel<D, FP16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>)));
-  rows_kernel<D, FP16><<<(unsigned)grid, THREADS, sizeof(Smem<D>), s>>>(p);
-  return check_launch("masked rows_kernel");
+  if (p.splits > 1 && p.splits <= MAX_CLUSTER) return launch_as<D, FP16, true>(p, grid, s);
+  return launch_as<D, FP16, false>(p, grid, s);
 }
 
 }  // namespace
 
-int rows_splits(long long units, long long kv_bound) {
-  const long long want = (TARGET_CTAS + units - 1) / units;
-  const long long most = (kv_bound + 127) / 128;  // two steps for each warp
-  return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, most), 64));
+int rows_splits(long long units, long long keys, bool single) {
+  const long long target = single ? TARGET_SINGLE : TARGET_SEVERAL;
+  const long long want = (target + units - 1) / units;
+  const long long splits = std::max<long long>(1, std::min<long long>(std::min<long long>(want, keys / MIN_KEYS), 64));
+  return (int)(splits > MAX_CLUSTER && keys <= MAX_CLUSTER * CLUSTER_KEYS ? MAX_CLUSTER : splits);
 }
 
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t s) {

@@ -263,8 +263,12 @@ __device__ __forceinline__ void rows_key_by_key(const Params& p, const int2* seg
   for (int r = 0; r < 32; ++r) {
     const int lo = __shfl_sync(0xffffffffu, row_lo, r), hi = __shfl_sync(0xffffffffu, row_hi, r);
     const int pos = __shfl_sync(0xffffffffu, row_pos, r);
-    if (!__shfl_sync(0xffffffffu, (int)row_valid, r)) continue;
     const long long row = row0 + r;
+    if (!__shfl_sync(0xffffffffu, (int)row_valid, r)) {
+      if (p.splits > 1 && row < p.q_rows && lane == 0)
+        p.part_ml[(split * p.q_rows + row) * p.heads + head] = make_float2(-INFINITY, NOT_MINE);
+      continue;
+    }
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + row * p.q_stride + (long long)head * D + lane * N;
     float qf[N], acc[N], m = -INFINITY, l = 0.f;
     for (int i = 0; i < N; ++i) qf[i] = widen<FP16>(q[i]), acc[i] = 0.f;
@@ -295,7 +299,7 @@ __device__ __forceinline__ void rows_key_by_key(const Params& p, const int2* seg
       for (int i = 0; i < N; ++i) out[i] = (uint16_t)pack2<FP16>(acc[i] * inv, 0.f);
     } else {
       // sums that the other splits raised by RAISE; here they are not, so the maximum says it
-      if (lane == 0) p.part_ml[at] = make_float2(m == -INFINITY ? m : m + RAISE<FP16>, l);
+      if (lane == 0) p.part_ml[at] = partial_ml(m + RAISE<FP16>, l, hi > lo);
       for (int i = 0; i < N; ++i) p.part[at * D + lane * N + i] = acc[i];
     }
   }
@@ -709,7 +713,8 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         if (!has_keys) m = -INFINITY, l = 0.f;
         const float inv = p.splits == 1 ? inverse_sum(l, has_keys) : 1.f;
         const long long at = (split * p.q_rows + row) * p.heads + head;
-        if (valid && p.splits > 1) p.part_ml[at] = make_float2(m, l);
+        if (p.splits > 1 && row < p.q_rows)
+          p.part_ml[at] = valid ? partial_ml(m, l, has_keys) : make_float2(-INFINITY, NOT_MINE);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t raw[32];
@@ -775,9 +780,9 @@ int launch_form(const Params& p, cudaStream_t s) {
 
 }  // namespace
 
-int tiles_splits(long long units, long long kv_bound) {
+int tiles_splits(long long units, long long keys) {
   const long long want = 148 / std::max<long long>(units, 1);
-  const long long most = kv_bound / (8 * BKV);  // eight tiles at least for each split
+  const long long most = 2 * keys / (8 * BKV);  // eight tiles at least for each split
   return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, most), 32));
 }
 
