@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_bf16.h>
 #include <stdint.h>
+#include <atomic>
 #include <string>
 
 #include "../../include/musc_b200.h"
@@ -37,6 +38,20 @@ int smem_optin(void);
 // Device address of the error word that kernels set when a bounded wait
 // expires (cached per device; nullptr on failure).
 int* device_error_ptr(void);
+
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device; done once per device.
+template <auto kernel>
+int opt_in_smem(size_t bytes) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return cuda_fail(err, "cudaGetDevice");
+  if (dev < 64 && done[dev].load(std::memory_order_acquire)) return MUSC_B200_OK;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err != cudaSuccess) return cuda_fail(err, "cudaFuncSetAttribute");
+  if (dev < 64) done[dev].store(true, std::memory_order_release);
+  return MUSC_B200_OK;
+}
 
 }  // namespace musc
 

@@ -190,8 +190,6 @@ extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args*
   p.splits = plan.splits;
   p.part = static_cast<float*>(a.workspace);
   p.part_ml = plan.bytes ? reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.ml_offset) : nullptr;
-  p.err = device_error_ptr();
-  if (!p.err) return fail(MUSC_B200_ERR_CUDA, "masked_attention: device error word unavailable");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool fp16 = a.dtype == MUSC_B200_F16;
   MUSC_TRY(plan.tiles ? tiles_launch(p, a.head_dim, fp16, s) : rows_launch(p, a.head_dim, fp16, s));

@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 
 template <int D, bool FP16, bool CLUSTER>
 int launch_as(const Params& p, long long grid, cudaStream_t s) {
-  const auto kernel = rows_kernel<D, FP16, CLUSTER>;
-  MUSC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>)));
+  constexpr auto kernel = rows_kernel<D, FP16, CLUSTER>;
+  MUSC_TRY(opt_in_smem<kernel>(sizeof(Smem<D>)));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)grid);
   config.blockDim = dim3(THREADS);

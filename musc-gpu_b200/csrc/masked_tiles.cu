@@ -758,7 +758,9 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
 }
 
 template <int D, bool FP16, bool CAP, bool BIAS>
-int launch(const Params& p, cudaStream_t s) {
+int launch(Params p, cudaStream_t s) {
+  p.err = device_error_ptr();
+  if (!p.err) return fail(MUSC_B200_ERR_CUDA, "masked_attention: device error word unavailable");
   const long long grid = (p.q_rows + ROWS - 1) / ROWS * p.heads * p.splits;
   if (grid > 0x7FFFFFFFLL) return fail(MUSC_B200_ERR_INVALID, "masked_attention: too many rows and heads");
   const int qw = p.heads * D, kw = p.kv_heads * D;
@@ -766,8 +768,8 @@ int launch(const Params& p, cudaStream_t s) {
   MUSC_TRY(make_token_map(&mq, p.q, p.q_rows, qw, p.q_rows > 1 ? p.q_stride : qw, FP16, BQ));
   MUSC_TRY(make_token_map(&mk, p.k, p.kv_rows, kw, p.kv_rows > 1 ? p.k_stride : kw, FP16, BKV));
   MUSC_TRY(make_token_map(&mv, p.v, p.kv_rows, kw, p.kv_rows > 1 ? p.v_stride : kw, FP16, BKV));
-  const auto kernel = tiles_kernel<D, FP16, CAP, BIAS>;
-  MUSC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_BYTES<D>));
+  constexpr auto kernel = tiles_kernel<D, FP16, CAP, BIAS>;
+  MUSC_TRY(opt_in_smem<kernel>(SMEM_BYTES<D>));
   kernel<<<(unsigned)grid, THREADS, SMEM_BYTES<D>, s>>>(mq, mk, mv, p);
   return check_launch("masked tiles_kernel");
 }

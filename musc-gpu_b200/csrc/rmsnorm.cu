@@ -9,20 +9,23 @@
 //
 // One read of x and delta, one write of x and y: memory bounds it.  A row's sums of squares
 // and h itself stay in 32 bits and in registers between the two uses, so h is normalised
-// before it is rounded to x's type.  A row goes to as many threads as give each at most four
-// runs of eight columns (a warp up to 1024 columns); eight columns of a run are consecutive,
-// which makes a 16-byte access of them and keeps a group of 128 columns on 16 neighbouring
-// lanes, whose shuffles find its amax.
+// before it is rounded to x's type.  A row goes to a warp (up to 1024 columns) or to a CTA of
+// 256 to 1024 threads; a CTA walks over rows and loads the next one before it works on this one, so that
+// loads are in flight during the reductions.  Where rows start on 16 bytes a thread takes runs of eight
+// consecutive columns: 16-byte accesses, and a group of 128 columns on 16 neighbouring lanes, whose
+// shuffles find its amax.  Otherwise consecutive threads take consecutive columns, a warp's 32 at a
+// time, and a group's amax is that of its slices of 32.
 #include "common.cuh"
 
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 namespace musc {
 namespace rms {
 
 constexpr int RUN = 8;        // consecutive columns of a thread
-constexpr int MAX_RUNS = 4;   // runs of a thread: 32 values in registers
-constexpr int MAX_THREADS = 1024;
+constexpr int MAX_CHANNELS = 32768;
 constexpr int WARP_ROWS = 4;  // rows of a CTA where a row is one warp's
 constexpr float E4M3_MAX = 448.0f;
 constexpr float MIN_SCALE = 1.17549435e-38f;  // 2^-126: its reciprocal is finite, rows of zeros stay zeros
@@ -39,27 +42,49 @@ struct Params {
   float eps;
 };
 
-// Eight columns from c on, those past the row as zeros.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_run(const T* row, int c, int channels, float (&v)[RUN]) {
+__device__ __forceinline__ float reciprocal(float x) {  // of a scale: off by 2^-23, e4m3 rounds at 2^-4
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Column of a thread's value i of run r.
+template <bool VEC>
+__device__ __forceinline__ int column(int r, int i, int tid, int threads) {
+  return VEC ? (r * threads + tid) * RUN + i : (r * RUN + i) * threads + tid;
+}
+
+// A run as it lies in memory.
+template <typename T>
+struct Raw {
+  uint4 w[sizeof(T) * RUN / 16];
+};
+
+template <typename E, bool VEC>
+__device__ __forceinline__ void load_run(Raw<E>& raw, const E* row, int r, int tid, int threads, int channels) {
   if (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 raw = *reinterpret_cast<const uint4*>(row + c);
-      const T* t = reinterpret_cast<const T*>(&raw);
+    const uint4* src = reinterpret_cast<const uint4*>(row + column<VEC>(r, 0, tid, threads));
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) v[i] = static_cast<float>(t[i]);
-    }
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) raw.w[i] = src[i];
   } else {
+    E* v = reinterpret_cast<E*>(raw.w);
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) v[i] = c + i < channels ? static_cast<float>(row[c + i]) : 0.f;
+    for (int i = 0; i < RUN; ++i) {
+      const int c = column<VEC>(r, i, tid, threads);
+      v[i] = c < channels ? row[c] : E(0.f);
+    }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T narrow(float v);
+template <typename E>
+__device__ __forceinline__ void widen(const Raw<E>& raw, float (&v)[RUN]) {
+  const E* t = reinterpret_cast<const E*>(raw.w);
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) v[i] = static_cast<float>(t[i]);
+}
+
+template <typename E>
+__device__ __forceinline__ E narrow(float v);
 template <>
 __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <>
@@ -67,40 +92,44 @@ __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_run(T* row, int c, int channels, const float (&v)[RUN]) {
+template <typename E, bool VEC>
+__device__ __forceinline__ void store_run(E* row, int r, int tid, int threads, int channels, const float (&v)[RUN]) {
   if (VEC) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      uint4 raw;
-      T* t = reinterpret_cast<T*>(&raw);
+    Raw<E> raw;
+    E* t = reinterpret_cast<E*>(raw.w);
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) t[i] = narrow<T>(v[i]);
-      *reinterpret_cast<uint4*>(row + c) = raw;
-    }
+    for (int i = 0; i < RUN; ++i) t[i] = narrow<E>(v[i]);
+    uint4* dst = reinterpret_cast<uint4*>(row + column<VEC>(r, 0, tid, threads));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(E) / 2; ++i) dst[i] = raw.w[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < RUN; ++i)
-      if (c + i < channels) row[c + i] = narrow<T>(v[i]);
+    for (int i = 0; i < RUN; ++i) {
+      const int c = column<VEC>(r, i, tid, threads);
+      if (c < channels) row[c] = narrow<E>(v[i]);
+    }
   }
 }
 
+// Eight values of e4m3, each value times its factor (one factor for a run of consecutive columns).
 template <bool VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t* row, int c, int channels, const float (&v)[RUN], float factor) {
+__device__ __forceinline__ void store_e4m3(uint8_t* row, int r, int tid, int threads, int channels, const float (&v)[RUN],
+                                           const float (&factor)[RUN]) {
   uint2 raw;
   __nv_fp8x2_storage_t* t = reinterpret_cast<__nv_fp8x2_storage_t*>(&raw);
 #pragma unroll
   for (int i = 0; i < RUN / 2; ++i)
-    t[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * factor, v[2 * i + 1] * factor), __NV_SATFINITE, __NV_E4M3);
+    t[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * factor[2 * i], v[2 * i + 1] * factor[2 * i + 1]), __NV_SATFINITE,
+                                    __NV_E4M3);
   if (VEC) {
-    *reinterpret_cast<uint2*>(row + c) = raw;
+    *reinterpret_cast<uint2*>(row + column<VEC>(r, 0, tid, threads)) = raw;
   } else {
     const uint8_t* b = reinterpret_cast<const uint8_t*>(&raw);
 #pragma unroll
-    for (int i = 0; i < RUN; ++i)
-      if (c + i < channels) row[c + i] = b[i];
+    for (int i = 0; i < RUN; ++i) {
+      const int c = column<VEC>(r, i, tid, threads);
+      if (c < channels) row[c] = b[i];
+    }
   }
 }
 
@@ -110,7 +139,7 @@ __device__ __forceinline__ float row_reduce(float v, Op op, float* shared) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (WARP) return v;
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (lane == 0) shared[threadIdx.x >> 5] = v;
   __syncthreads();
   v = shared[lane < warps ? lane : 0];
@@ -122,106 +151,186 @@ __device__ __forceinline__ float row_reduce(float v, Op op, float* shared) {
   return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// WARP: a row is one warp's, WARP_ROWS rows a CTA; otherwise a row is the CTA's.
-template <typename XT, typename DT, bool VEC, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * WARP_ROWS : MAX_THREADS) add_rmsnorm_kernel(const Params p) {
-  __shared__ float shared[2][32];
-  const long long row = WARP ? (long long)blockIdx.x * WARP_ROWS + (threadIdx.x >> 5) : (long long)blockIdx.x;
-  if (row >= p.rows) return;  // uniform over a row's threads
+// A row is a warp's, WARP_ROWS rows a CTA, or a CTA's; a thread has at most RUNS runs of it.
+// CTAs that fit an SM, by which the compiler bounds the registers of a thread.  A vectorised row of a
+// warp: three of 128 threads with the weights in registers (5480 rows of 1024 in 12.0 us; with four, or
+// with the weights read again for every row, 13 us).  A vectorised row of a CTA: 64 registers, so that
+// two of 512 fit, weights read again (16389 rows of 4096 in 75 us; with 83 registers and the weights kept 93 us).
+template <bool VEC, int T>
+constexpr int MIN_CTAS = T == 0 || T == 512 ? 2 : T == 1024 ? 1 : T == 256 ? 4 : 3;
+
+// T: threads of a row, 0: the CTA's, at most 512.
+template <typename XT, typename DT, bool VEC, int T, int RUNS>
+__global__ void __launch_bounds__(T == 32 ? 32 * WARP_ROWS : T ? T : 512, MIN_CTAS<VEC, T>) add_rmsnorm_kernel(const Params p) {
+  constexpr bool WARP = T == 32;
+  __shared__ float shared[2][2][32];  // [parity of the row][sum or amax][warp]
+  __shared__ float slice_top[VEC ? 1 : (WARP ? WARP_ROWS : 1)][VEC ? 1 : (WARP ? 32 : 1024)];  // of 32 columns; then of groups
+  const int threads = T ? T : blockDim.x;
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const int step = (WARP ? 32 : blockDim.x) * RUN;
-  XT* x = static_cast<XT*>(p.x) + row * p.x_stride;
-  const DT* delta = static_cast<const DT*>(p.delta) + row * p.delta_stride;
-  float v[MAX_RUNS][RUN];
-  float sum = 0.f;
+  const int sub = WARP ? threadIdx.x >> 5 : 0;
+  const long long step = WARP ? (long long)gridDim.x * WARP_ROWS : (long long)gridDim.x;
+  long long row = WARP ? (long long)blockIdx.x * WARP_ROWS + sub : (long long)blockIdx.x;
+  const auto mine = [&](int r) { return column<VEC>(r, 0, tid, threads) < p.channels; };  // the run has a column of the row
+  Raw<XT> next_x[RUNS];
+  Raw<DT> next_d[RUNS];
+  const auto load = [&](long long at) {
+    const XT* x = static_cast<const XT*>(p.x) + at * p.x_stride;
+    const DT* d = static_cast<const DT*>(p.delta) + at * p.delta_stride;
 #pragma unroll
-  for (int r = 0; r < MAX_RUNS; ++r) {
-    const int c = r * step + tid * RUN;
-    if (c < p.channels) load_run<XT, VEC>(x, c, p.channels, v[r]);
+    for (int r = 0; r < RUNS; ++r)
+      if (mine(r)) load_run<XT, VEC>(next_x[r], x, r, tid, threads, p.channels);
+    if (p.delta) {
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r)
+        if (mine(r)) load_run<DT, VEC>(next_d[r], d, r, tid, threads, p.channels);
+    }
+  };
+  constexpr bool AHEAD = VEC && (RUNS == 2 || WARP);  // elsewhere registers for a second row would cost more than it gives
+  if (AHEAD && row < p.rows) load(row);
+  constexpr bool KEEP = VEC && WARP;  // the thread's weights, the same for every row
+  Raw<float> weight[KEEP ? RUNS : 1];
+  if (KEEP) {
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r)
+      if (mine(r)) load_run<float, VEC>(weight[KEEP ? r : 0], p.weight, r, tid, threads, p.channels);
   }
-  if (p.delta) {
+  for (int parity = 0; row < p.rows; row += step, parity ^= 1) {  // uniform over a row's threads
+    if (!AHEAD) load(row);
+    float v[RUNS][RUN];
+    XT* x = static_cast<XT*>(p.x) + row * p.x_stride;
+    float sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < MAX_RUNS; ++r) {
-      const int c = r * step + tid * RUN;
-      if (c < p.channels) {
-        float d[RUN];
-        load_run<DT, VEC>(delta, c, p.channels, d);
+    for (int r = 0; r < RUNS; ++r) {
+      if (mine(r)) {
+        widen(next_x[r], v[r]);
+        if (p.delta) {
+          float d[RUN];
+          widen(next_d[r], d);
 #pragma unroll
-        for (int i = 0; i < RUN; ++i) v[r][i] += d[i];
-        store_run<XT, VEC>(x, c, p.channels, v[r]);
+          for (int i = 0; i < RUN; ++i) v[r][i] += d[i];
+          store_run<XT, VEC>(x, r, tid, threads, p.channels, v[r]);
+        }
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) sum = fmaf(v[r][i], v[r][i], sum);
+      } else {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) v[r][i] = 0.f;
       }
     }
-  }
+    if (AHEAD && row + step < p.rows) load(row + step);
+    sum = row_reduce<WARP>(sum, [](float a, float b) { return a + b; }, shared[parity][0]);
+    const float rstd = rsqrtf(sum / (float)p.channels + p.eps);
+    float top = 0.f;  // of the row
 #pragma unroll
-  for (int r = 0; r < MAX_RUNS; ++r) {
-    if (r * step + tid * RUN < p.channels) {
+    for (int r = 0; r < RUNS; ++r) {
+      if (mine(r)) {
+        if (!KEEP) load_run<float, VEC>(weight[0], p.weight, r, tid, threads, p.channels);
+        float w[RUN];
+        widen(weight[KEEP ? r : 0], w);
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) sum = fmaf(v[r][i], v[r][i], sum);
+        for (int i = 0; i < RUN; ++i) {
+          v[r][i] = v[r][i] * rstd * w[i];
+          if (!VEC && column<VEC>(r, i, tid, threads) >= p.channels) v[r][i] = 0.f;  // no value, also where rstd is not finite
+        }
+        const long long at = row * p.out_stride;
+        if (p.out_dtype == MUSC_B200_F32) store_run<float, VEC>(static_cast<float*>(p.out) + at, r, tid, threads, p.channels, v[r]);
+        else if (p.out_dtype == MUSC_B200_F16) store_run<__half, VEC>(static_cast<__half*>(p.out) + at, r, tid, threads, p.channels, v[r]);
+        else if (p.out_dtype == MUSC_B200_BF16) store_run<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(p.out) + at, r, tid, threads, p.channels, v[r]);
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) top = fmaxf(top, fabsf(v[r][i]));
+      }
     }
-  }
-  sum = row_reduce<WARP>(sum, [](float a, float b) { return a + b; }, shared[0]);
-  const float rstd = rsqrtf(sum / (float)p.channels + p.eps);
-  float top = 0.f;  // of the row
+    if (p.out_dtype != MUSC_B200_E4M3) continue;
+    uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_stride;
+    float* scales = p.scales + row * p.groups;
+    const auto scale_of = [](float m) { return fmaxf(m * (1.f / E4M3_MAX), MIN_SCALE); };
+    float factor[RUN];
+    if (p.group == 0) {
+      top = row_reduce<WARP>(top, [](float a, float b) { return fmaxf(a, b); }, shared[parity][1]);
+      const float scale = scale_of(top);
+      if (tid == 0) scales[0] = scale;
 #pragma unroll
-  for (int r = 0; r < MAX_RUNS; ++r) {
-    const int c = r * step + tid * RUN;
-    if (c < p.channels) {
-      float w[RUN];
-      load_run<float, VEC>(p.weight, c, p.channels, w);
+      for (int i = 0; i < RUN; ++i) factor[i] = reciprocal(scale);
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) v[r][i] = v[r][i] * rstd * w[i];
-      if (p.out_dtype == MUSC_B200_F32) store_run<float, VEC>(static_cast<float*>(p.out) + row * p.out_stride, c, p.channels, v[r]);
-      else if (p.out_dtype == MUSC_B200_F16) store_run<__half, VEC>(static_cast<__half*>(p.out) + row * p.out_stride, c, p.channels, v[r]);
-      else if (p.out_dtype == MUSC_B200_BF16) store_run<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(p.out) + row * p.out_stride, c, p.channels, v[r]);
+      for (int r = 0; r < RUNS; ++r)
+        if (mine(r)) store_e4m3<VEC>(out, r, tid, threads, p.channels, v[r], factor);
+    } else if (VEC) {
+      const int lanes = p.group / RUN;  // 4 to 32 neighbouring lanes hold a group
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r) {
+        if (r * threads * RUN >= p.channels) break;  // uniform over the row's threads
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) m = fmaxf(m, fabsf(v[r][i]));
+        for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float scale = scale_of(m);
+        if (mine(r)) {
+          if (tid % lanes == 0) scales[column<VEC>(r, 0, tid, threads) / p.group] = scale;
+#pragma unroll
+          for (int i = 0; i < RUN; ++i) factor[i] = reciprocal(scale);
+          store_e4m3<VEC>(out, r, tid, threads, p.channels, v[r], factor);
+        }
+      }
     } else {
+      // Slice k, columns 32 k to 32 k + 31, is a warp's; a group is group / 32 slices.
+      const int warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
 #pragma unroll
-      for (int i = 0; i < RUN; ++i) v[r][i] = 0.f;
-    }
+      for (int r = 0; r < RUNS; ++r)
 #pragma unroll
-    for (int i = 0; i < RUN; ++i) top = fmaxf(top, fabsf(v[r][i]));
-  }
-  if (p.out_dtype != MUSC_B200_E4M3) return;
-  uint8_t* out = static_cast<uint8_t*>(p.out) + row * p.out_stride;
-  float* scales = p.scales + row * p.groups;
-  if (p.group == 0) {
-    top = row_reduce<WARP>(top, [](float a, float b) { return fmaxf(a, b); }, shared[1]);
-    const float scale = fmaxf(top / E4M3_MAX, MIN_SCALE);
-    if (tid == 0) scales[0] = scale;
-#pragma unroll
-    for (int r = 0; r < MAX_RUNS; ++r) {
-      const int c = r * step + tid * RUN;
-      if (c < p.channels) store_e4m3<VEC>(out, c, p.channels, v[r], 1.0f / scale);
-    }
-  } else {
-    const int lanes = p.group / RUN;  // 4 to 32 neighbouring lanes hold a group
-#pragma unroll
-    for (int r = 0; r < MAX_RUNS; ++r) {
-      const int c = r * step + tid * RUN;
-      if (r * step >= p.channels) break;  // uniform over the row's threads
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < RUN; ++i) m = fmaxf(m, fabsf(v[r][i]));
-      for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float scale = fmaxf(m / E4M3_MAX, MIN_SCALE);
-      if (c < p.channels) {
-        if (tid % lanes == 0) scales[c / p.group] = scale;
-        store_e4m3<VEC>(out, c, p.channels, v[r], 1.0f / scale);
+        for (int i = 0; i < RUN; ++i) {
+          const float m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(v[r][i]), 0.f))));
+          if (lane == 0) slice_top[sub][(r * RUN + i) * warps + warp] = m;
+        }
+      const int in_group = p.group / 32, slices = RUNS * RUN * warps;
+      const auto sync = [] {
+        if (WARP) __syncwarp();
+        else __syncthreads();
+      };
+      sync();
+      // A thread's share of the groups: scales out, reciprocals in the place of each group's first slice.
+      for (int g = tid; g < p.groups; g += threads) {
+        float m = 0.f;
+        for (int k = g * in_group; k < min((g + 1) * in_group, slices); ++k) m = fmaxf(m, slice_top[sub][k]);
+        const float scale = scale_of(m);
+        scales[g] = scale;
+        slice_top[sub][g * in_group] = reciprocal(scale);
       }
+      sync();
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r) {
+#pragma unroll
+        for (int i = 0; i < RUN; ++i) factor[i] = slice_top[sub][((r * RUN + i) * warps + warp) & ~(in_group - 1)];
+        store_e4m3<VEC>(out, r, tid, threads, p.channels, v[r], factor);
+      }
+      sync();  // the next row's slices come after these have been read
     }
   }
 }
 
+constexpr int THREADS_PER_SM = 4096;  // of a grid: about two waves
+
+template <typename XT, typename DT, bool VEC, int T, int RUNS>
+int launch_as(const Params& p, int threads, cudaStream_t s) {
+  const long long ctas = T == 32 ? (p.rows + WARP_ROWS - 1) / WARP_ROWS : p.rows;
+  // As many rows for every CTA, few enough CTAs that most of them walk over several.
+  const long long most = (long long)sm_count() * std::max(1, THREADS_PER_SM / threads);
+  const long long each = (ctas + most - 1) / most;
+  add_rmsnorm_kernel<XT, DT, VEC, T, RUNS><<<(unsigned)((ctas + each - 1) / each), threads, 0, s>>>(p);
+  return check_launch("add_rmsnorm_kernel");
+}
+
 template <typename XT, typename DT, bool VEC>
 int launch_rows(const Params& p, cudaStream_t s) {
-  if (p.channels <= 32 * RUN * MAX_RUNS) {
-    const long long grid = (p.rows + WARP_ROWS - 1) / WARP_ROWS;
-    add_rmsnorm_kernel<XT, DT, VEC, true><<<(unsigned)grid, 32 * WARP_ROWS, 0, s>>>(p);
-  } else {
-    int threads = 64;
-    while (threads * RUN * MAX_RUNS < p.channels) threads *= 2;
-    add_rmsnorm_kernel<XT, DT, VEC, false><<<(unsigned)p.rows, threads, 0, s>>>(p);
+  if (p.channels <= 32 * 4 * RUN) return launch_as<XT, DT, VEC, 32, 4>(p, 32 * WARP_ROWS, s);
+  const int runs = (p.channels + RUN - 1) / RUN;
+  if constexpr (VEC) {
+    if (runs <= 2 * 512) return launch_as<XT, DT, VEC, 0, 2>(p, ((runs + 1) / 2 + 31) / 32 * 32, s);
+  } else {  // a column of its own for every value: their distances are constants
+    if (runs <= 2 * 256) return launch_as<XT, DT, VEC, 256, 2>(p, 256, s);
+    if (runs <= 2 * 512) return launch_as<XT, DT, VEC, 512, 2>(p, 512, s);
   }
-  return check_launch("add_rmsnorm_kernel");
+  if (runs <= 2 * 1024) return launch_as<XT, DT, VEC, 1024, 2>(p, 1024, s);
+  return launch_as<XT, DT, VEC, 1024, 4>(p, 1024, s);
 }
 
 template <typename XT>
@@ -248,7 +357,7 @@ extern "C" int musc_b200_add_rmsnorm(void* x, int x_dtype, const void* delta, in
     return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: x and delta must be f32, f16 or bf16");
   if (!wide(out_dtype) && out_dtype != MUSC_B200_E4M3)
     return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: out dtype must be f32, f16, bf16 or e4m3");
-  if (rows < 0 || rows > 0x7FFFFFFFLL || channels <= 0 || channels > MAX_THREADS * RUN * MAX_RUNS)
+  if (rows < 0 || rows > 0x7FFFFFFFLL || channels <= 0 || channels > MAX_CHANNELS)
     return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: 0 <= rows < 2^31 and 1 <= channels <= 32768");
   if (!(eps >= 0.f)) return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: eps must not be negative");
   if (group != 0 && (out_dtype != MUSC_B200_E4M3 || (group != 32 && group != 64 && group != 128 && group != 256)))

@@ -8,6 +8,7 @@ the CPU: a missing library or a non-sm_100 device raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Sequence
@@ -511,8 +512,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
 
 def _forward_only(what: str, *tensors: torch.Tensor | None) -> None:
     """These operators have no backward pass: refuse inputs whose gradient would be lost."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f'{what}: no gradient is computed; call it under torch.no_grad() or detach the inputs')
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f'{what}: no gradient is computed; call it under torch.no_grad() or detach the inputs')
 
 
 def _on_device(what: str, device: torch.device, **tensors: torch.Tensor | None) -> None:
@@ -521,23 +524,42 @@ def _on_device(what: str, device: torch.device, **tensors: torch.Tensor | None) 
             raise ValueError(f'{what}: {name} must be on {device}')
 
 
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _guard(device: torch.device):
+    """``torch.cuda.device(device)`` where it is not the current one already (entering it takes longer than
+    the smallest of these calls)."""
+    return _NO_GUARD if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
 def _token_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
     """``(rows, row stride, rows between batch items)`` of a token-major ``(T, W)`` or ``(B, L, W)`` tensor."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    shape, stride = t.shape, t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         raise ValueError(f'{what}: {name} must be contiguous in its last dimension')
-    if t.ndim == 2:
-        return t.shape[0], (t.stride(0) if t.shape[0] > 1 else t.shape[1]), t.shape[0]
-    b, length, width = t.shape
+    if len(shape) == 2:
+        rows, width = shape
+        return rows, (stride[0] if rows > 1 else width), rows
+    b, length, width = shape
     if b * length == 0:
         return 0, width, length
     if length == 1:
-        return b, (t.stride(0) if b > 1 else width), 1
+        return b, (stride[0] if b > 1 else width), 1
     if b == 1:
-        return length, t.stride(1), length
-    if t.stride(1) <= 0 or t.stride(0) % t.stride(1) != 0 or t.stride(0) // t.stride(1) < length:
+        return length, stride[1], length
+    if stride[1] <= 0 or stride[0] % stride[1] != 0 or stride[0] // stride[1] < length:
         raise ValueError(f'{what}: the batch items of {name} must lie a whole number of rows apart')
-    pitch = t.stride(0) // t.stride(1)
-    return (b - 1) * pitch + length, t.stride(1), pitch
+    pitch = stride[0] // stride[1]
+    return (b - 1) * pitch + length, stride[1], pitch
 
 
 def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, kv_heads: int | None = None, *,
@@ -598,30 +620,27 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     if q.ndim == 3 and (q_pitch != q.shape[1] or v_pitch != kv_pitch):
         raise ValueError('attention_masked: batch items of q must follow each other, those of k and v lie equally far apart')
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError('attention_masked: out must have the shape and type of q')
-    _, out_stride, out_pitch = _token_rows(what, 'out', out)
-    if q.ndim == 3 and out_pitch != q_pitch:
-        raise ValueError('attention_masked: batch items of out must follow each other')
+        out, out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), heads * head_dim
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError('attention_masked: out must have the shape and type of q')
+        _, out_stride, out_pitch = _token_rows(what, 'out', out)
+        if q.ndim == 3 and out_pitch != q_pitch:
+            raise ValueError('attention_masked: batch items of out must follow each other')
     args = _lib.MaskedAttentionArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), dtype=_DTYPES[q.dtype], heads=heads,
-        kv_heads=kv_heads, head_dim=head_dim, q_rows=q_rows, kv_rows=kv_rows, q_stride=q_stride, k_stride=k_stride,
-        v_stride=v_stride, out_stride=out_stride, documents=docs, causal=int(causal),
-        q_offsets=offsets.data_ptr() if packed else None, kv_offsets=kv_offsets.data_ptr() if packed else None,
-        kv_lengths=kv_lengths.data_ptr() if kv_lengths is not None else None,
-        prefix=prefix.data_ptr() if prefix is not None else None,
-        q_len=0 if packed else q.shape[1], kv_len=0 if packed else k.shape[1], kv_pitch=0 if packed else kv_pitch,
-        slopes=slopes.data_ptr() if slopes is not None else None,
-        scale=head_dim ** -0.5 if scale is None else scale, softcap=softcap)
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _DTYPES[q.dtype], heads, kv_heads, head_dim, q_rows,
+        kv_rows, q_stride, k_stride, v_stride, out_stride, docs, causal, _at(offsets), _at(kv_offsets), _at(kv_lengths),
+        _at(prefix), 0 if packed else q.shape[1], 0 if packed else k.shape[1], 0 if packed else kv_pitch, _at(slopes),
+        head_dim ** -0.5 if scale is None else scale, softcap)
     lib = _lib.lib()
-    with torch.cuda.device(dev):
+    with _guard(dev):
         ws_bytes = lib.musc_b200_masked_attention_bytes(ctypes.byref(args))
         if ws_bytes:
             ws = _aligned_empty(ws_bytes, dev, 256)
             args.workspace, args.workspace_bytes = ws.data_ptr(), ws_bytes
-        st = lib.musc_b200_masked_attention(ctypes.byref(args), _stream(dev))
-        _lib.check(st, 'musc_b200_masked_attention')
+        st = lib.musc_b200_masked_attention(ctypes.byref(args), _raw_stream(dev))
+        if st != _lib.OK:
+            _lib.check(st, 'musc_b200_masked_attention')
     return out
 
 
@@ -662,8 +681,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     _require_cuda(q, what)
     _forward_only(what, q, k, positions, frequencies)
     dev = q.device
-    outs = (None, None) if out is None else out
-    _on_device(what, dev, k=k, positions=positions, frequencies=frequencies, axis=axis, q_out=outs[0], k_out=outs[1])
+    _on_device(what, dev, k=k, positions=positions, frequencies=frequencies, axis=axis)
+    if out is not None:
+        _on_device(what, dev, q_out=out[0], k_out=out[1])
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
         raise ValueError('rotary: q and k must share one type, float32, float16 or bfloat16')
     kv_heads = heads if kv_heads is None else kv_heads
@@ -679,30 +699,37 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
         raise ValueError('rotary: frequencies must be a contiguous (pairs,) float32 tensor')
     if axis.dtype != torch.int32 or axis.shape != frequencies.shape or not axis.is_contiguous():
         raise ValueError('rotary: axis must be a contiguous int32 tensor of the shape of frequencies')
-    ins = [q] if k is None else [q, k]
-    if out is None:
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=dev) for t in ins]
-    else:
-        outs = list(out)[:len(ins)]
-        for t, o in zip(ins, outs):
-            if o is None or o.shape != t.shape or o.dtype != t.dtype:
-                raise ValueError('rotary: out must be (q_out, k_out) of the shapes and type of q and k')
-    strides = []
-    for name, t in zip(('q', 'k', 'q_out', 'k_out') if k is not None else ('q', 'q_out'), ins + outs):
-        rows, stride, pitch = _token_rows(what, name, t)
+
+    def stride(name, t):
+        _, row, pitch = _token_rows(what, name, t)
         if t.ndim == 3 and pitch != t.shape[1]:
             raise ValueError(f'rotary: batch items of {name} must follow each other')
-        strides.append(stride)
+        return row
+
+    q_out, k_out = (None, None) if out is None else out
+    q_stride, k_stride = stride('q', q), 0 if k is None else stride('k', k)
+    if out is None:
+        q_out, q_out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), heads * head_dim
+        if k is not None:
+            k_out, k_out_stride = torch.empty(k.shape, dtype=k.dtype, device=dev), kv_heads * head_dim
+    else:
+        for t, o in ((q, q_out), (k, k_out)):
+            if t is not None and (o is None or o.shape != t.shape or o.dtype != t.dtype):
+                raise ValueError('rotary: out must be (q_out, k_out) of the shapes and type of q and k')
+        q_out_stride = stride('q_out', q_out)
+        if k is not None:
+            k_out_stride = stride('k_out', k_out)
+    if k is None:
+        kv_heads, k_out, k_out_stride = 0, None, 0
     tokens = q.numel() // q.shape[-1] if q.shape[-1] else 0
-    n = len(ins)
-    with torch.cuda.device(dev):
+    with _guard(dev):
         st = _lib.lib().musc_b200_rotary(
-            _ptr(q), _ptr(k), _ptr(outs[0]), _ptr(outs[1] if n == 2 else None), _DTYPES[q.dtype], tokens, heads,
-            kv_heads if n == 2 else 0, head_dim, strides[0], strides[1] if n == 2 else 0, strides[n],
-            strides[n + 1] if n == 2 else 0, _ptr(positions), int(positions.dtype == torch.float32),
-            positions.shape[-1], _ptr(frequencies), _ptr(axis), frequencies.numel(), int(adjacent), _stream(dev))
-        _lib.check(st, 'musc_b200_rotary')
-    return outs[0], (outs[1] if n == 2 else None)
+            q.data_ptr(), _at(k), q_out.data_ptr(), _at(k_out), _DTYPES[q.dtype], tokens, heads, kv_heads, head_dim, q_stride,
+            k_stride, q_out_stride, k_out_stride, positions.data_ptr(), positions.dtype == torch.float32,
+            positions.shape[-1], frequencies.data_ptr(), axis.data_ptr(), frequencies.numel(), adjacent, _raw_stream(dev))
+        if st != _lib.OK:
+            _lib.check(st, 'musc_b200_rotary')
+    return q_out, k_out
 
 
 # --------------------------------------------------------------------------- RMS norm
@@ -759,12 +786,13 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
             strides.append(t.stride(0))
         else:
             raise ValueError(f'add_rmsnorm: {name} must be contiguous, or (rows, C) with contiguous rows')
-    with torch.cuda.device(dev):
+    with _guard(dev):
         st = _lib.lib().musc_b200_add_rmsnorm(
-            _ptr(x), _DTYPES[x.dtype], _ptr(delta), _DTYPES[delta.dtype] if delta is not None else 0, _ptr(weight),
-            float(eps), _ptr(out), _lib.E4M3 if eight else _DTYPES[out_dtype], _ptr(scales if eight else None), group,
-            rows, c, strides[0], strides[1], strides[2], _stream(dev))
-        _lib.check(st, 'musc_b200_add_rmsnorm')
+            x.data_ptr(), _DTYPES[x.dtype], _at(delta), _DTYPES[delta.dtype] if delta is not None else 0, weight.data_ptr(),
+            eps, out.data_ptr(), _lib.E4M3 if eight else _DTYPES[out_dtype], scales.data_ptr() if eight else None, group,
+            rows, c, strides[0], strides[1], strides[2], _raw_stream(dev))
+        if st != _lib.OK:
+            _lib.check(st, 'musc_b200_add_rmsnorm')
     return (out, scales) if eight else out
 
 
