@@ -12,7 +12,7 @@
 // it.  The angles are the same for all heads of a token: a CTA takes a few tokens, puts
 // their cosines and sines into shared memory once (tokens x pairs of them, instead of a
 // table in memory that would be read beside q and k), and then streams q and k in 16-byte
-// vectors, two items of a thread in flight.  The angle is formed in 64 bits and reduced to a
+// vectors, the first of them on their way while the angles are computed.  The angle is formed in 64 bits and reduced to a
 // fraction of a turn before it is rounded to 32: a position of 100,000 has an angle whose
 // 32-bit rounding is 4e-3 of a radian.  A token takes pairs 64-bit products, 1/40 of the
 // kernel's instructions at 16 + 16 heads of 64.
@@ -24,8 +24,12 @@ namespace musc {
 namespace rotary {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TOKENS = 16;   // tokens per CTA
-constexpr int ITEMS_PER_CTA = 1024;  // items (two vectors) a CTA should have before it takes fewer tokens
+constexpr int MAX_TABLE = 32 * 1024;  // bytes of a CTA's cosines and sines
+// A CTA takes tokens until it has this many items (of two vectors), eight a thread, and loads them
+// one by one: 65001 tokens of 20 heads of 128 take 123 us; with two or four loads in flight per
+// thread the registers cost more CTAs than that gives (133, 157 us), with half the items the
+// angles weigh more (127 us).
+constexpr int ITEMS_PER_CTA = THREADS * 8;
 
 struct Params {
   const void* in[2];
@@ -39,7 +43,13 @@ struct Params {
   int head_dim, pairs, axes;
   int tokens_per_cta;
   int float_positions;
+  uint32_t token_magic, head_magic;  // ceil(2^32 / items of a token, of a head); 0: divide
 };
+
+// n / d with magic = ceil(2^32 / d), exact while n * d < 2^32.
+__device__ __forceinline__ int divide(int n, int d, uint32_t magic) {
+  return magic ? (int)__umulhi((uint32_t)n, magic) : n / d;
+}
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) {
@@ -83,29 +93,27 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Params p) {
   constexpr int V = VEC ? 16 / (int)sizeof(T) : 1;
   const long long t0 = (long long)blockIdx.x * p.tokens_per_cta;
   const int n_tok = (int)min((long long)p.tokens_per_cta, p.tokens - t0);
-  fill_angles(p, t0, n_tok, table);
-  __syncthreads();
   // Items of a head: turned ones of V pairs each, then passed-through ones of 2 V elements.
   const int turned = p.pairs / V;
   const int rest = p.head_dim - 2 * p.pairs;
   const int per_head = turned + (rest + 2 * V - 1) / (2 * V);
   const int per_token = per_head * (p.heads[0] + p.heads[1]);
   const int total = per_token * n_tok;
-  constexpr int U = 2;
-  for (int e0 = threadIdx.x; e0 < total; e0 += THREADS * U) {
+  constexpr int U = VEC ? 1 : 4;
+  for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < total; e0 += THREADS * U) {  // uniform over the CTA
     Vec<T> a[U], b[U];
     T* dst[U];
-    int second[U];   // offset of the item's second half from its first; 0: there is none
+    int second[U];   // offset of the item's second half from its first
     int angle[U];    // index of its first pair's angle, -1: passes through
-    int count[U];
+    int count[U];    // halves
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int e = e0 + u * THREADS;
       count[u] = 0;
       if (e < total) {
-        const int t = e / per_token;
+        const int t = divide(e, per_token, p.token_magic);
         const int in_token = e - t * per_token;
-        int head = in_token / per_head;
+        int head = divide(in_token, per_head, p.head_magic);
         const int item = in_token - head * per_head;
         const int which = head >= p.heads[0] ? 1 : 0;
         if (which) head -= p.heads[0];
@@ -134,6 +142,10 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(const Params p) {
           if (count[u] == 2) b[u].v[0] = src[second[u]];
         }
       }
+    }
+    if (e0 == (int)threadIdx.x) {  // while the first items are on their way
+      fill_angles(p, t0, n_tok, table);
+      __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -255,12 +267,15 @@ extern "C" int musc_b200_rotary(const void* q, const void* k, void* q_out, void*
   const int per_head = pairs / v + (head_dim - 2 * pairs + 2 * v - 1) / (2 * v);
   const long long per_token = (long long)per_head * (heads + kv_heads);
   // More tokens in a CTA while one has few items, but not fewer than two CTAs per SM.
-  long long n = (ITEMS_PER_CTA + per_token - 1) / per_token;
+  long long n = ITEMS_PER_CTA / per_token;
   n = std::min<long long>(n, std::max<long long>(1, tokens / (2 * sm_count())));
-  p.tokens_per_cta = (int)std::min<long long>(std::max<long long>(n, 1), MAX_TOKENS);
+  p.tokens_per_cta = (int)std::max<long long>(1, std::min<long long>(n, MAX_TABLE / ((long long)pairs * sizeof(float2))));
   const long long grid = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
   if (grid > 0x7FFFFFFFLL || per_token * p.tokens_per_cta > 0x3FFFFFFFLL)
     return fail(MUSC_B200_ERR_INVALID, "rotary: too many tokens or heads");
+  const long long most = std::max<long long>(per_token * p.tokens_per_cta, per_token) * per_token;
+  p.token_magic = most < (1LL << 32) && per_token > 1 ? (uint32_t)(((1ULL << 32) + per_token - 1) / per_token) : 0;
+  p.head_magic = most < (1LL << 32) && per_head > 1 ? (uint32_t)(((1ULL << 32) + per_head - 1) / per_head) : 0;
   const size_t smem = (size_t)p.tokens_per_cta * pairs * sizeof(float2);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == MUSC_B200_F32) return launch<float>(p, adjacent != 0, vec, (unsigned)grid, smem, s);
