@@ -16,6 +16,8 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (unit >= p.q_rows * p.heads) return;
   const int lane = threadIdx.x & 31;
+  const long long row = unit / p.heads;
+  if (p.q_offsets && (row < __ldg(p.q_offsets) || row >= __ldg(p.q_offsets + p.documents))) return;  // of no document
   const long long per_split = p.q_rows * p.heads;
   float m[2], l[2], w[2];
 #pragma unroll
@@ -24,7 +26,6 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
     const float2 ml = s < p.splits ? p.part_ml[s * per_split + unit] : make_float2(-INFINITY, 0.f);
     m[i] = ml.x, l[i] = ml.y;
   }
-  if (__any_sync(0xffffffffu, l[0] == NOT_MINE)) return;
   const float common = warp_max(fmaxf(m[0], m[1]));
   float total = 0.f;
 #pragma unroll
@@ -48,7 +49,6 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
     for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(weight, o[i], acc[i]);
   }
   const float inv = inverse_sum(total, common != -INFINITY);
-  const long long row = unit / p.heads;
   const int head = (int)(unit - row * p.heads);
   uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.out_stride + (long long)head * D + lane * (D / 32);
 #pragma unroll
@@ -90,7 +90,7 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   // heads of a key head (up to 16), reading its keys again for every row.
   plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
   if (plan.tiles)
-    plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a));
+    plan.splits = tiles_splits(((a.q_rows + 255) / 256) * a.heads, mean_keys(a));
   else
     plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), mean_keys(a), a.q_rows <= a.documents);
   if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {
@@ -192,6 +192,10 @@ extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args*
   p.part_ml = plan.bytes ? reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.ml_offset) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool fp16 = a.dtype == MUSC_B200_F16;
+  p.aligned = tiles_aligned(p), p.row_tiles = 0;
+  const long long row_tiles = tiles_of_rows(p);
+  if (row_tiles > 0x7FFFFFFF) return invalid("too many rows");
+  p.row_tiles = (int)row_tiles;
   MUSC_TRY(plan.tiles ? tiles_launch(p, a.head_dim, fp16, s) : rows_launch(p, a.head_dim, fp16, s));
   if (plan.bytes > 0) MUSC_TRY(combine_launch(p, a.head_dim, fp16, s));
   return MUSC_B200_OK;

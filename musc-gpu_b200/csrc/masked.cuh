@@ -43,6 +43,8 @@ struct Params {
   float* part;
   float2* part_ml;
   int* err;
+  // Tile kernel: grid of row tiles, and whether documents begin their own (masked_tiles.cu).
+  int row_tiles, aligned;
 };
 
 // Keys [lo, hi) of the packed keys that a row sees, and the key its own position falls on.
@@ -131,12 +133,10 @@ template <bool FP16>
 constexpr float RAISE = FP16 ? 6.f : 0.f;
 
 // A split's partial result of a row and head: its reference maximum and its sum.  The maximum of a
-// row that sees keys is finite even where it met none of them; (-inf, 0) says that it sees no key,
-// (-inf, -1) that it belongs to no document and is not written.
+// row that sees keys is finite even where it met none of them; (-inf, 0) says that it sees no key.
 __device__ __forceinline__ float2 partial_ml(float m, float l, bool any_key) {
   return make_float2(any_key ? fmaxf(m, -FLT_MAX) : -INFINITY, l);
 }
-constexpr float NOT_MINE = -1.f;
 
 // Weight of a split's partial sums against the row's common maximum.
 __device__ __forceinline__ float split_weight(float m, float common) {
@@ -157,6 +157,8 @@ int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int rows_splits(long long units, long long keys, bool single);  // single: one row for each document
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int tiles_splits(long long units, long long keys);
+bool tiles_aligned(const Params& p);
+long long tiles_of_rows(const Params& p);  // row tiles of the grid
 int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 
 }  // namespace masked

@@ -115,11 +115,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   const int head0 = kv_head * p.group + block * HEADS;
   const int n_heads = min(HEADS, p.group - block * HEADS);
   const int doc = find_document_warp(p, row);
-  if (doc < 0) {  // uniform over the CTA and its cluster
-    if (!CLUSTER && p.splits > 1 && threadIdx.x < n_heads)
-      p.part_ml[(split * p.q_rows + row) * p.heads + head0 + threadIdx.x] = make_float2(-INFINITY, NOT_MINE);
-    return;
-  }
+  if (doc < 0) return;  // uniform over the CTA and its cluster
   const Interval iv = row_interval(p, doc, row);
   // This split's share of the interval, in whole steps.
   const long long steps = (iv.hi - iv.lo + KEYS - 1) / KEYS;

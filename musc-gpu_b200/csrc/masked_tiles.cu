@@ -58,9 +58,14 @@ struct Smem {
   uint64_t p_full[2][2], o_full[2][2];  // per half and buffer of P
   uint64_t drained[2];
   union {
-    int offsets[SHARED_DOCS + 1];  // while the rows' documents are looked up
-    int2 segments[ROWS];           // then: key ranges [x, y) that the CTA walks
+    struct {                         // while the rows' documents are looked up
+      int offsets[SHARED_DOCS + 1];
+      uint16_t run[SHARED_DOCS];     // first document of the run that a document belongs to
+    };
+    int2 segments[ROWS];             // then: key ranges [x, y) that the CTA walks
   };
+  int scan[2][THREADS / 32];         // of the warps: last run begun, row tiles
+  int tile_doc, tile_row0, total_tiles;
   int lo[ROWS], hi[ROWS], doc[ROWS];
   uint32_t starts[ROWS / 32];      // rows that begin another document than the row before
   int hull[2][2];                  // per half: first key and end of all its rows' keys
@@ -264,11 +269,7 @@ __device__ __forceinline__ void rows_key_by_key(const Params& p, const int2* seg
     const int lo = __shfl_sync(0xffffffffu, row_lo, r), hi = __shfl_sync(0xffffffffu, row_hi, r);
     const int pos = __shfl_sync(0xffffffffu, row_pos, r);
     const long long row = row0 + r;
-    if (!__shfl_sync(0xffffffffu, (int)row_valid, r)) {
-      if (p.splits > 1 && row < p.q_rows && lane == 0)
-        p.part_ml[(split * p.q_rows + row) * p.heads + head] = make_float2(-INFINITY, NOT_MINE);
-      continue;
-    }
+    if (!__shfl_sync(0xffffffffu, (int)row_valid, r)) continue;
     const uint16_t* q = static_cast<const uint16_t*>(p.q) + row * p.q_stride + (long long)head * D + lane * N;
     float qf[N], acc[N], m = -INFINITY, l = 0.f;
     for (int i = 0; i < N; ++i) qf[i] = widen<FP16>(q[i]), acc[i] = 0.f;
@@ -318,13 +319,11 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   volatile int* abort_flag = &sm.abort_flag;
   // Heads change fastest (those of a group share K and V in L2), then the row tiles -- the
   // last rows first, since with a causal mask they see the most keys -- then the splits.
-  const int n_row_tiles = (int)((p.q_rows + ROWS - 1) / ROWS);
   int unit = blockIdx.x;
   const int head = unit % p.heads;
   unit /= p.heads;
-  const int row_tile = n_row_tiles - 1 - unit % n_row_tiles, split = unit / n_row_tiles;
+  const int row_tile = p.row_tiles - 1 - unit % p.row_tiles, split = unit / p.row_tiles;
   const int kv_head = head / p.group;
-  const long long row0 = (long long)row_tile * ROWS;
 
   if (threadIdx.x == 256) {
     tc::mbar_init(tc::smem_u32(&sm.q_full), 1);
@@ -356,15 +355,86 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     tc::tmem_relinquish();
   }
 
-  // ------------------------------------------------ the rows' intervals and the CTA's walk
+  // ------------------------------------------------ the CTA's rows, their intervals and its walk
   const bool shared_offsets = p.q_offsets && p.documents <= SHARED_DOCS;
   if (shared_offsets)
     for (int i = threadIdx.x; i <= p.documents; i += THREADS) sm.offsets[i] = __ldg(p.q_offsets + i);
+  if (threadIdx.x == 0) sm.tile_doc = -1;
+  tc::fence_before_sync();
   __syncthreads();
+  tc::fence_after_sync();
+  // First row, and the run of documents that the tile is cut from (-1: all rows).
+  long long row0 = (long long)row_tile * ROWS;
+  int run = -1;
+  if (p.aligned && shared_offsets) {
+    // A document of ROWS rows and more is a run of its own, shorter ones that follow each other are
+    // one run.  Runs are cut into tiles from their first row on: a document's tiles are those that
+    // begin in it.  Each thread takes PER documents; two scans over the threads.
+    constexpr int PER = (SHARED_DOCS + THREADS - 1) / THREADS;
+    const int d0 = threadIdx.x * PER;
+    const auto rows_of = [&](int d) { return max(sm.offsets[d + 1] - sm.offsets[d], 0); };
+    int begun = -1;
+    for (int d = d0; d < min(d0 + PER, p.documents); ++d)
+      if (d == 0 || rows_of(d) >= ROWS || rows_of(d - 1) >= ROWS) begun = d;
+    int before = begun;  // inclusive, then exclusive, maximum over the threads
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before = max(before, other);
+    }
+    if (lane == 31) sm.scan[0][warp] = before;
+    before = __shfl_up_sync(0xffffffffu, before, 1);
+    if (lane == 0) before = -1;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before = max(before, sm.scan[0][w]);
+    int tiles[PER], sum = 0, at = before;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int d = d0 + i;
+      tiles[i] = 0;
+      if (d < p.documents) {
+        if (d == 0 || rows_of(d) >= ROWS || rows_of(d - 1) >= ROWS) at = d;
+        sm.run[d] = (uint16_t)at;
+        const int from = max(sm.offsets[d] - sm.offsets[at], 0);
+        tiles[i] = (from + rows_of(d) + ROWS - 1) / ROWS - (from + ROWS - 1) / ROWS;
+        sum += tiles[i];
+      }
+    }
+    int first = sum;  // inclusive, then exclusive, sum over the threads
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, first, o);
+      if (lane >= o) first += other;
+    }
+    if (lane == 31) sm.scan[1][warp] = first;
+    first -= sum;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) first += sm.scan[1][w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (row_tile >= first && row_tile < first + tiles[i]) {
+        const int d = d0 + i, start = sm.offsets[sm.run[d]];
+        sm.tile_doc = d;
+        sm.tile_row0 = start + ((max(sm.offsets[d] - start, 0) + ROWS - 1) / ROWS + row_tile - first) * ROWS;
+      }
+      first += tiles[i];
+    }
+    __syncthreads();
+    run = sm.tile_doc < 0 ? -2 : sm.run[sm.tile_doc];
+    row0 = sm.tile_row0;
+  } else if (p.aligned) {
+    const int per_doc = (int)((p.q_len + ROWS - 1) / ROWS);
+    run = row_tile / per_doc;
+    row0 = run * p.q_len + (long long)(row_tile - run * per_doc) * ROWS;
+  }
+  if (run == -2) {  // the grid's bound was higher than the documents' tiles
+    if (warp == SOFTMAX_WARPS + 1) tc::tmem_dealloc(sm.tmem_base, TMEM_COLS);
+    return;
+  }
   int doc = -1, lo = 0, hi = 0, pos = 0;
   if (threadIdx.x < ROWS) {
     const long long row = row0 + threadIdx.x;
-    if (row < p.q_rows) {
+    if (row >= 0 && row < p.q_rows) {
       if (!shared_offsets) {
         doc = find_document(p, row);
       } else if (row >= sm.offsets[0] && row < sm.offsets[p.documents]) {
@@ -376,6 +446,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         }
         doc = a;
       }
+      if (doc >= 0 && run >= 0 && (shared_offsets ? sm.run[doc] : doc) != run) doc = -1;  // another tile's
     }
     if (doc >= 0) {
       const Interval iv = row_interval(p, doc, row);
@@ -434,9 +505,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     sm.n_segments = n;
     sm.n_tiles = tiles;
   }
-  tc::fence_before_sync();
   __syncthreads();
-  tc::fence_after_sync();
   const uint32_t tmem_base = sm.tmem_base;
   const int first_tile = (int)((long long)sm.n_tiles * split / p.splits);
   const int last_tile = (int)((long long)sm.n_tiles * (split + 1) / p.splits);
@@ -713,8 +782,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         if (!has_keys) m = -INFINITY, l = 0.f;
         const float inv = p.splits == 1 ? inverse_sum(l, has_keys) : 1.f;
         const long long at = (split * p.q_rows + row) * p.heads + head;
-        if (p.splits > 1 && row < p.q_rows)
-          p.part_ml[at] = valid ? partial_ml(m, l, has_keys) : make_float2(-INFINITY, NOT_MINE);
+        if (valid && p.splits > 1) p.part_ml[at] = partial_ml(m, l, has_keys);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           uint32_t raw[32];
@@ -761,7 +829,7 @@ template <int D, bool FP16, bool CAP, bool BIAS>
 int launch(Params p, cudaStream_t s) {
   p.err = device_error_ptr();
   if (!p.err) return fail(MUSC_B200_ERR_CUDA, "masked_attention: device error word unavailable");
-  const long long grid = (p.q_rows + ROWS - 1) / ROWS * p.heads * p.splits;
+  const long long grid = (long long)p.row_tiles * p.heads * p.splits;
   if (grid > 0x7FFFFFFFLL) return fail(MUSC_B200_ERR_INVALID, "masked_attention: too many rows and heads");
   const int qw = p.heads * D, kw = p.kv_heads * D;
   CUtensorMap mq, mk, mv;
@@ -786,6 +854,21 @@ int tiles_splits(long long units, long long keys) {
   const long long want = 148 / std::max<long long>(units, 1);
   const long long most = 2 * keys / (8 * BKV);  // eight tiles at least for each split
   return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, most), 32));
+}
+
+// Documents begin tiles of their own (long ones; runs of short ones share them) where they have 64 rows in
+// the mean: a tile that holds the end of one long document and the start of another walks both one's keys.
+bool tiles_aligned(const Params& p) {
+  return p.q_offsets ? p.documents <= SHARED_DOCS && p.q_rows >= 64LL * p.documents : p.q_len >= ROWS;
+}
+
+// A bound of the row tiles: the documents' lengths are only known on the device.  Every run after the first
+// adds at most one tile to the packed rows' own; there are at most two for every document of ROWS rows, and one.
+long long tiles_of_rows(const Params& p) {
+  const long long packed = (p.q_rows + ROWS - 1) / ROWS;
+  if (!p.aligned) return packed;
+  if (!p.q_offsets) return p.documents * ((p.q_len + ROWS - 1) / ROWS);
+  return packed + std::min<long long>(p.documents, 2 * (p.q_rows / ROWS) + 1) - 1;
 }
 
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t s) {

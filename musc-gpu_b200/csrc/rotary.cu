@@ -24,7 +24,7 @@ namespace musc {
 namespace rotary {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TABLE = 32 * 1024;  // bytes of a CTA's cosines and sines
+constexpr int MAX_TOKENS = 16;  // tokens of a CTA: 32 KB of cosines and sines at most
 // A CTA takes tokens until it has this many items (of two vectors), eight a thread, and loads them
 // one by one: 65001 tokens of 20 heads of 128 take 123 us; with two or four loads in flight per
 // thread the registers cost more CTAs than that gives (133, 157 us), with half the items the
@@ -269,7 +269,7 @@ extern "C" int musc_b200_rotary(const void* q, const void* k, void* q_out, void*
   // More tokens in a CTA while one has few items, but not fewer than two CTAs per SM.
   long long n = ITEMS_PER_CTA / per_token;
   n = std::min<long long>(n, std::max<long long>(1, tokens / (2 * sm_count())));
-  p.tokens_per_cta = (int)std::max<long long>(1, std::min<long long>(n, MAX_TABLE / ((long long)pairs * sizeof(float2))));
+  p.tokens_per_cta = (int)std::max<long long>(1, std::min<long long>(n, MAX_TOKENS));
   const long long grid = (tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
   if (grid > 0x7FFFFFFFLL || per_token * p.tokens_per_cta > 0x3FFFFFFFLL)
     return fail(MUSC_B200_ERR_INVALID, "rotary: too many tokens or heads");
