@@ -66,7 +66,7 @@ struct Smem {
   };
   int scan[2][THREADS / 32];         // of the warps: last run begun, row tiles
   int tile_doc, tile_row0, total_tiles;
-  int lo[ROWS], hi[ROWS], doc[ROWS];
+  int lo[ROWS], hi[ROWS];
   uint32_t starts[ROWS / 32];      // rows that begin another document than the row before
   int hull[2][2];                  // per half: first key and end of all its rows' keys
   int common[2];                   // the keys that all rows with keys see: from, to
@@ -365,8 +365,34 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   tc::fence_after_sync();
   // First row, and the run of documents that the tile is cut from (-1: all rows).
   long long row0 = (long long)row_tile * ROWS;
-  int run = -1;
-  if (p.aligned && shared_offsets) {
+  int run = -1, run_end = 0x7FFFFFFF;  // documents [run, run_end)
+  if (p.aligned && shared_offsets && p.documents <= 32) {
+    // As below, by every warp for itself: a lane for each document.
+    const int d = min(lane, p.documents), from = sm.offsets[d], to = sm.offsets[min(d + 1, p.documents)];
+    const int rows = max(to - from, 0), rows_before = __shfl_up_sync(0xffffffffu, rows, 1);
+    const bool begins = lane < p.documents && (lane == 0 || rows >= ROWS || rows_before >= ROWS);
+    const uint32_t runs = __ballot_sync(0xffffffffu, begins);
+    const int mine = 31 - __clz(runs & (0xFFFFFFFFu >> (31 - lane)));  // lane 0 begins one: there is a document
+    const int start = __shfl_sync(0xffffffffu, from, mine), in_run = max(from - start, 0);
+    const int tiles = lane < p.documents ? (in_run + rows + ROWS - 1) / ROWS - (in_run + ROWS - 1) / ROWS : 0;
+    int first = tiles;  // inclusive, then exclusive, sum
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, first, o);
+      if (lane >= o) first += other;
+    }
+    first -= tiles;
+    const uint32_t owner = __ballot_sync(0xffffffffu, row_tile >= first && row_tile < first + tiles);
+    if (owner == 0) {
+      run = -2;
+    } else {
+      const int d_tile = __ffs(owner) - 1;
+      run = __shfl_sync(0xffffffffu, mine, d_tile);
+      const uint32_t later = run < 31 ? runs & (0xFFFFFFFEu << run) : 0u;
+      run_end = later ? __ffs(later) - 1 : p.documents;
+      row0 = __shfl_sync(0xffffffffu, start + ((in_run + ROWS - 1) / ROWS + row_tile - first) * ROWS, d_tile);
+    }
+  } else if (p.aligned && shared_offsets) {
     // A document of ROWS rows and more is a run of its own, shorter ones that follow each other are
     // one run.  Runs are cut into tiles from their first row on: a document's tiles are those that
     // begin in it.  Each thread takes PER documents; two scans over the threads.
@@ -422,37 +448,55 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
     __syncthreads();
     run = sm.tile_doc < 0 ? -2 : sm.run[sm.tile_doc];
     row0 = sm.tile_row0;
+    run_end = -1;  // not known, but which run a document belongs to
   } else if (p.aligned) {
     const int per_doc = (int)((p.q_len + ROWS - 1) / ROWS);
     run = row_tile / per_doc;
     row0 = run * p.q_len + (long long)(row_tile - run * per_doc) * ROWS;
+    run_end = run + 1;
   }
   if (run == -2) {  // the grid's bound was higher than the documents' tiles
     if (warp == SOFTMAX_WARPS + 1) tc::tmem_dealloc(sm.tmem_base, TMEM_COLS);
     return;
   }
+  if (threadIdx.x == 256) {  // Q is on its way while the keys are looked up
+    const uint32_t full = tc::smem_u32(&sm.q_full);
+    tc::mbar_arrive_expect_tx(full, 2 * NB * Q_BLOCK);
+    for (int h = 0; h < 2; ++h)
+      for (int b = 0; b < NB; ++b)
+        tc::tma_load_2d(tc::smem_u32(sm.q[h][b]), &map_q, head * D + b * 64, (int)row0 + h * BQ, full);
+  }
+  // Document of a row of this tile; -1: of none, or another tile's.
+  const auto document_of = [&](long long row) {
+    if (row < 0 || row >= p.q_rows) return -1;
+    int d = -1;
+    if (!shared_offsets) {
+      d = find_document(p, row);
+    } else if (row >= sm.offsets[0] && row < sm.offsets[p.documents]) {
+      int a = 0, b = p.documents;
+      while (b - a > 1) {
+        const int mid = (a + b) >> 1;
+        if (sm.offsets[mid] <= row) a = mid;
+        else b = mid;
+      }
+      d = a;
+    }
+    const bool here = run < 0 || d < 0 || (run_end < 0 ? sm.run[d] == run : d >= run && d < run_end);
+    return here ? d : -1;
+  };
   int doc = -1, lo = 0, hi = 0, pos = 0;
   if (threadIdx.x < ROWS) {
     const long long row = row0 + threadIdx.x;
-    if (row >= 0 && row < p.q_rows) {
-      if (!shared_offsets) {
-        doc = find_document(p, row);
-      } else if (row >= sm.offsets[0] && row < sm.offsets[p.documents]) {
-        int a = 0, b = p.documents;
-        while (b - a > 1) {
-          const int mid = (a + b) >> 1;
-          if (sm.offsets[mid] <= row) a = mid;
-          else b = mid;
-        }
-        doc = a;
-      }
-      if (doc >= 0 && run >= 0 && (shared_offsets ? sm.run[doc] : doc) != run) doc = -1;  // another tile's
-    }
+    doc = document_of(row);
+    int doc_before = __shfl_up_sync(0xffffffffu, doc, 1);
+    if (lane == 0) doc_before = threadIdx.x == 0 ? -2 : document_of(row - 1);
+    const uint32_t bits = __ballot_sync(0xffffffffu, doc != doc_before);
+    if (lane == 0) sm.starts[warp] = bits;
     if (doc >= 0) {
       const Interval iv = row_interval(p, doc, row);
       lo = (int)iv.lo, hi = (int)iv.hi, pos = (int)iv.pos;
     }
-    sm.lo[threadIdx.x] = lo, sm.hi[threadIdx.x] = hi, sm.doc[threadIdx.x] = doc;
+    sm.lo[threadIdx.x] = lo, sm.hi[threadIdx.x] = hi;
     const int first = __reduce_min_sync(0xffffffffu, hi > lo ? lo : 0x7FFFFFFF);
     const int end = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
     const int all_from = __reduce_max_sync(0xffffffffu, hi > lo ? lo : 0);
@@ -463,12 +507,6 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
       atomicMax(&sm.common[0], all_from);
       atomicMin(&sm.common[1], all_to);
     }
-  }
-  __syncthreads();
-  if (threadIdx.x < ROWS) {
-    const bool start = threadIdx.x == 0 || sm.doc[threadIdx.x] != sm.doc[threadIdx.x - 1];
-    const uint32_t bits = __ballot_sync(0xffffffffu, start);
-    if (lane == 0) sm.starts[warp] = bits;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -514,12 +552,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   if (warp >= SOFTMAX_WARPS) {
    if (warp == SOFTMAX_WARPS) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && n_tiles > 0) {
-      const uint32_t qf = tc::smem_u32(&sm.q_full);
-      tc::mbar_arrive_expect_tx(qf, 2 * NB * Q_BLOCK);
-      for (int h = 0; h < 2; ++h)
-        for (int b = 0; b < NB; ++b)
-          tc::tma_load_2d(tc::smem_u32(sm.q[h][b]), &map_q, head * D + b * 64, (int)row0 + h * BQ, qf);
+    if (lane == 0) {
       Walk walk(sm.segments, first_tile, last_tile);
       int begin, end, issued = 0;
       while (walk.next(begin, end)) {
@@ -534,7 +567,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
         ++issued;
       }
       // Let every copy this thread issued land before the CTA can exit.
-      drain(qf, 0);
+      drain(tc::smem_u32(&sm.q_full), 0);
       for (int t = max(issued - NS, 0); t < issued; ++t) drain(tc::smem_u32(&sm.full[t % NS]), (uint32_t)(t / NS) & 1u);
     }
    } else if (warp <= SOFTMAX_WARPS + 2) {
