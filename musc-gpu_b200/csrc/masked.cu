@@ -90,7 +90,7 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   // heads of a key head (up to 16), reading its keys again for every row.
   plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
   if (plan.tiles)
-    plan.splits = tiles_splits(((a.q_rows + 255) / 256) * a.heads, mean_keys(a));
+    plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a), a.causal != 0);
   else
     plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), mean_keys(a), a.q_rows <= a.documents);
   if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {

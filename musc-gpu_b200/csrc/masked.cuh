@@ -156,7 +156,7 @@ constexpr int MAX_CLUSTER = 8;  // up to so many splits the row kernel joins by 
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int rows_splits(long long units, long long keys, bool single);  // single: one row for each document
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
-int tiles_splits(long long units, long long keys);
+int tiles_splits(long long units, long long keys, bool causal);
 bool tiles_aligned(const Params& p);
 long long tiles_of_rows(const Params& p);  // row tiles of the grid
 int combine_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);

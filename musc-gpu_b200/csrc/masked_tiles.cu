@@ -883,10 +883,15 @@ int launch_form(const Params& p, cudaStream_t s) {
 
 }  // namespace
 
-int tiles_splits(long long units, long long keys) {
-  const long long want = 148 / std::max<long long>(units, 1);
-  const long long most = 2 * keys / (8 * BKV);  // eight tiles at least for each split
-  return (int)std::max<long long>(1, std::min<long long>(std::min<long long>(want, most), 32));
+// One wave of CTAs (148 SMs): a second one costs more than the finer division gives (2048 tokens of 16
+// heads in 37 us, with two waves 57).  With a causal mask the last rows' CTAs take twice the mean, and long
+// ones are divided for that: 8192 tokens of 4 heads in 78 us, in one piece 118; 2753 tokens of
+// 16 heads in 67 us, divided 78.
+int tiles_splits(long long units, long long keys, bool causal) {
+  units = std::max<long long>(units, 1);
+  long long splits = std::min<long long>(148 / units, keys / 256);
+  if (causal) splits = std::max(splits, std::min<long long>((2 * 148 + units / 2) / units, keys / 2048));
+  return (int)std::max<long long>(1, std::min<long long>(splits, 32));
 }
 
 // Documents begin tiles of their own (long ones; runs of short ones share them) where they have 64 rows in
