@@ -682,51 +682,49 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     _forward_only(what, q, k, positions, frequencies)
     dev = q.device
     _on_device(what, dev, k=k, positions=positions, frequencies=frequencies, axis=axis)
-    if out is not None:
-        _on_device(what, dev, q_out=out[0], k_out=out[1])
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
         raise ValueError('rotary: q and k must share one type, float32, float16 or bfloat16')
     kv_heads = heads if kv_heads is None else kv_heads
-    if heads <= 0 or kv_heads <= 0 or q.shape[-1] % heads != 0:
+    *batch, width = q.shape
+    if heads <= 0 or kv_heads <= 0 or width % heads != 0:
         raise ValueError('rotary: heads must divide the width of q')
-    head_dim = q.shape[-1] // heads
-    if q.ndim not in (2, 3) or (k is not None and k.shape != (*q.shape[:-1], kv_heads * head_dim)):
+    head_dim = width // heads
+    if len(batch) not in (1, 2) or (k is not None and k.shape != (*batch, kv_heads * head_dim)):
         raise ValueError('rotary: expected q (T, heads*D) or (B, L, heads*D) and k (..., kv_heads*D) of as many tokens')
-    if positions.dtype not in (torch.int32, torch.float32) or positions.ndim != q.ndim or \
-            positions.shape[:-1] != q.shape[:-1] or positions.shape[-1] < 1 or not positions.is_contiguous():
+    *tokens_of, axes = positions.shape if positions.ndim else (0,)
+    if positions.dtype not in (torch.int32, torch.float32) or tokens_of != batch or axes < 1 or not positions.is_contiguous():
         raise ValueError('rotary: positions must be a contiguous (..., axes) int32 or float32 tensor with the tokens of q')
     if frequencies.dtype != torch.float32 or frequencies.ndim != 1 or not frequencies.is_contiguous():
         raise ValueError('rotary: frequencies must be a contiguous (pairs,) float32 tensor')
     if axis.dtype != torch.int32 or axis.shape != frequencies.shape or not axis.is_contiguous():
         raise ValueError('rotary: axis must be a contiguous int32 tensor of the shape of frequencies')
 
-    def stride(name, t):
+    def row_stride(name, t):
         _, row, pitch = _token_rows(what, name, t)
-        if t.ndim == 3 and pitch != t.shape[1]:
+        if len(batch) == 2 and pitch != batch[1]:
             raise ValueError(f'rotary: batch items of {name} must follow each other')
         return row
 
-    q_out, k_out = (None, None) if out is None else out
-    q_stride, k_stride = stride('q', q), 0 if k is None else stride('k', k)
+    q_stride, k_stride = row_stride('q', q), 0 if k is None else row_stride('k', k)
+    k_out, k_out_stride = None, kv_heads * head_dim
     if out is None:
-        q_out, q_out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), heads * head_dim
+        q_out, q_out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), width
         if k is not None:
-            k_out, k_out_stride = torch.empty(k.shape, dtype=k.dtype, device=dev), kv_heads * head_dim
+            k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
     else:
-        for t, o in ((q, q_out), (k, k_out)):
+        _on_device(what, dev, q_out=out[0], k_out=out[1])
+        for t, o in ((q, out[0]), (k, out[1])):
             if t is not None and (o is None or o.shape != t.shape or o.dtype != t.dtype):
                 raise ValueError('rotary: out must be (q_out, k_out) of the shapes and type of q and k')
-        q_out_stride = stride('q_out', q_out)
+        q_out, q_out_stride = out[0], row_stride('q_out', out[0])
         if k is not None:
-            k_out_stride = stride('k_out', k_out)
-    if k is None:
-        kv_heads, k_out, k_out_stride = 0, None, 0
-    tokens = q.numel() // q.shape[-1] if q.shape[-1] else 0
+            k_out, k_out_stride = out[1], row_stride('k_out', out[1])
     with _guard(dev):
         st = _lib.lib().musc_b200_rotary(
-            q.data_ptr(), _at(k), q_out.data_ptr(), _at(k_out), _DTYPES[q.dtype], tokens, heads, kv_heads, head_dim, q_stride,
-            k_stride, q_out_stride, k_out_stride, positions.data_ptr(), positions.dtype == torch.float32,
-            positions.shape[-1], frequencies.data_ptr(), axis.data_ptr(), frequencies.numel(), adjacent, _raw_stream(dev))
+            q.data_ptr(), _at(k), q_out.data_ptr(), _at(k_out), _DTYPES[q.dtype], math.prod(batch), heads,
+            kv_heads if k is not None else 0, head_dim, q_stride, k_stride, q_out_stride, k_out_stride,
+            positions.data_ptr(), positions.dtype == torch.float32, axes, frequencies.data_ptr(), axis.data_ptr(),
+            frequencies.shape[0], adjacent, _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_rotary')
     return q_out, k_out
