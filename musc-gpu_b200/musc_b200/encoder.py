@@ -24,6 +24,7 @@ Weights use the reference's ``state_dict`` names, so a trained CLIP
 """
 from __future__ import annotations
 
+import itertools
 import math
 from typing import Sequence
 
@@ -34,10 +35,17 @@ from . import ops
 
 
 class VisionEncoder:
-    """Weights + forward of an open_clip ``VisionTransformer`` (no patch dropout/pooler)."""
+    """Weights + forward of an open_clip ``VisionTransformer`` (no patch dropout/pooler).
+
+    ``rotary``: the base of two-axis rotary positions for towers that have them: every block's
+    queries and keys turn by their patch's row and column (:func:`musc_b200.ops.rotary`; the class token
+    stands at (0, 0)), half of a head's pairs each.  ``positional_embedding`` is then optional, and
+    :meth:`forward_packed` takes images of differing sizes.
+    """
 
     def __init__(self, state: dict, image_size: int = 518, patch_size: int = 14, width: int = 1024,
-                 layers: int = 24, heads: int = 16, device='cuda', compute_dtype=torch.float16):
+                 layers: int = 24, heads: int = 16, device='cuda', compute_dtype=torch.float16,
+                 rotary: float | None = None):
         if width // heads != 64:
             raise ValueError('the b200 attention kernel needs head_dim 64')
         if compute_dtype not in (torch.float16, torch.bfloat16):
@@ -51,7 +59,8 @@ class VisionEncoder:
         bf = lambda k: state[k].to(dev, compute_dtype).contiguous()
         self.conv_w = bf('conv1.weight').reshape(width, -1)          # (width, 3*p*p)
         self.cls = f32('class_embedding')
-        self.pos = f32('positional_embedding')
+        self.pos = f32('positional_embedding') if rotary is None or 'positional_embedding' in state else None
+        self.rotary = None if rotary is None else ops.rotary_frequencies([16, 16], rotary, device=dev)
         self.ln_pre = (f32('ln_pre.weight'), f32('ln_pre.bias'))
         self.blocks = []
         for i in range(layers):
@@ -123,8 +132,18 @@ class VisionEncoder:
         # conv1 with stride = kernel = patch: a GEMM over non-overlapping patches
         patches = images.reshape(b, 3, g, p, g, p).permute(0, 2, 4, 1, 3, 5).reshape(b, g * g, 3 * p * p)
         x = F.linear(patches.to(lp), self.conv_w).float()                       # (B, g^2, width)
-        x = torch.cat([self.cls.expand(b, 1, w), x], dim=1) + self.pos
+        x = torch.cat([self.cls.expand(b, 1, w), x], dim=1)
+        if self.pos is not None:
+            x = x + self.pos
         x = F.layer_norm(x, (w,), *self.ln_pre).contiguous()
+        positions = None if self.rotary is None else _grid_positions([(g, g)] * b, x.device).view(b, 1 + g * g, 2)
+        x, tokens = self._run_blocks(x, out_layers, positions,
+                                     lambda q, k, v: ops.attention(q, k, v, self.heads))
+        return self._pool(x[:, 0]), [tokens[l] for l in out_layers]
+
+    def _run_blocks(self, x: torch.Tensor, out_layers: Sequence[int], positions, attend):
+        """The blocks over ``x`` ``(..., width)`` fp32; returns it and the tokens after ``out_layers``."""
+        lp, w = self.dtype, self.width
         keep = set(int(l) for l in out_layers)
         tokens = {}
         # Each residual add is fused with the LayerNorm that follows it (ops.add_layernorm:
@@ -136,15 +155,62 @@ class VisionEncoder:
             if idx - 1 in keep:
                 tokens[idx - 1] = x.clone()                              # x after block idx - 1
             qkv = self._linear(h, blk['in_w'], blk['in_b'])                      # (B, L, 3w) 16-bit
-            a = ops.attention(qkv[..., :w], qkv[..., w:2 * w], qkv[..., 2 * w:], self.heads)
+            q, k, v = qkv[..., :w], qkv[..., w:2 * w], qkv[..., 2 * w:]
+            if positions is not None:
+                ops.rotary(q, k, positions, *self.rotary, self.heads, out=(q, k))
+            a = attend(q, k, v)
             h = ops.add_layernorm(x, self._linear(a, blk['out_w'], blk['out_b']), *blk['ln_2'], out_dtype=lp)
             h = F.gelu(self._linear(h, blk['fc_w'], blk['fc_b']))       # evaluated in fp32 by torch
             pending = self._linear(h, blk['proj_w'], blk['proj_b'])
         x = x + pending                                                  # the last block's residual
         if len(self.blocks) in keep:
             tokens[len(self.blocks)] = x
-        pooled = F.layer_norm(x[:, 0], (w,), *self.ln_post) @ self.proj
-        return pooled, [tokens[l] for l in out_layers]
+        return x, tokens
+
+    def _pool(self, cls: torch.Tensor) -> torch.Tensor:
+        return F.layer_norm(cls, (self.width,), *self.ln_post) @ self.proj
+
+    def forward_packed(self, images: Sequence[torch.Tensor], out_layers: Sequence[int]):
+        """Images ``(3, H_i, W_i)`` of differing sizes (multiples of the patch size) in one pass:
+        their tokens follow each other in one sequence, and each attends to its own image's only
+        (``ops.attention_masked``).  For towers with rotary positions.  Returns ``(pooled (N, out_dim) fp32,
+        [[tokens of image i (1 + patches, width) fp32] per layer])``.
+        """
+        if self.rotary is None or self.pos is not None:
+            raise ValueError('forward_packed: the tower needs rotary positions and no learned grid')
+        if not images:
+            raise ValueError('forward_packed: no images')
+        p, w = self.patch_size, self.width
+        grids, patches = [], []
+        for im in images:
+            if im.ndim != 3 or im.shape[0] != 3 or im.shape[1] % p or im.shape[2] % p or im.numel() == 0:
+                raise ValueError(f'forward_packed: images must be (3, H, W) with H and W multiples of {p}')
+            gh, gw = im.shape[1] // p, im.shape[2] // p
+            grids.append((gh, gw))
+            patches.append(im.reshape(3, gh, p, gw, p).permute(1, 3, 0, 2, 4).reshape(gh * gw, 3 * p * p))
+        flag = torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction
+        torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = False
+        try:
+            parts = F.linear(torch.cat(patches).to(self.dtype), self.conv_w).float().split([gh * gw for gh, gw in grids])
+            x = torch.cat([t for part in parts for t in (self.cls.view(1, w), part)])
+            x = F.layer_norm(x, (w,), *self.ln_pre).contiguous()
+            lengths = [1 + gh * gw for gh, gw in grids]
+            starts = [0, *itertools.accumulate(lengths)]
+            offsets = torch.tensor(starts, dtype=torch.int32, device=x.device)
+            x, tokens = self._run_blocks(x, out_layers, _grid_positions(grids, x.device),
+                                         lambda q, k, v: ops.attention_masked(q, k, v, self.heads, offsets=offsets))
+            return self._pool(x[offsets[:-1].long()]), [list(tokens[l].split(lengths)) for l in out_layers]
+        finally:
+            torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = flag
+
+
+def _grid_positions(grids: Sequence[tuple[int, int]], device) -> torch.Tensor:
+    """(row, column) of every token of images with a class token before their patches, ``(tokens, 2)`` int32."""
+    parts = []
+    for gh, gw in grids:
+        patch = torch.arange(gh * gw, dtype=torch.int32, device=device)
+        parts.append(F.pad(torch.stack([patch // gw, patch % gw], 1), (0, 0, 1, 0)))
+    return torch.cat(parts)
 
 
 def random_vit_state(seed: int = 0, image_size: int = 518, patch_size: int = 14, width: int = 1024,
