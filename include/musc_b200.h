@@ -388,7 +388,7 @@ int musc_b200_add_layernorm(float* x, const void* delta, int delta_dtype, const 
  * 0: one scale) or over each group of 32, 64, 128 or 256 columns (a row or
  * group of zeros: 2^-126).  1 <= channels <= 32768, any alignment (16-byte
  * vectors are used where every row starts on 16 bytes and channels % 8 == 0);
- * the memory ranges of x, delta, out and scales must not overlap.  rows == 0 does nothing. */
+ * the memory ranges of x, delta, weight, out and scales must not overlap.  rows == 0 does nothing. */
 int musc_b200_add_rmsnorm(void* x, int x_dtype, const void* delta, int delta_dtype, const float* weight,
                           float eps, void* out, int out_dtype, float* scales, int group, long long rows,
                           int channels, long long x_stride, long long delta_stride, long long out_stride,
@@ -435,6 +435,7 @@ int musc_b200_rotary(const void* q, const void* k, void* q_out, void* k_out, int
  * d * kv_pitch on.  kv_lengths [documents] (nullable): keys in use at the start of
  * each slot.  Values outside the tensors are clamped to them.  Query rows
  * outside every document are not written.
+ * scale from 1e-20 to 1e20, softcap 0 or from 1e-15 to 1e15.
  * out must not overlap q, k or v.  workspace: musc_b200_masked_attention_bytes
  * (0 if none is needed), 256-byte aligned, free for reuse once the stream has
  * passed the call. */

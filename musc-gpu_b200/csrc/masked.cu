@@ -110,8 +110,9 @@ int check_args(const musc_b200_masked_attention_args& a) {
   if (a.q_rows < 0 || a.kv_rows < 0 || a.q_rows > 0x7FFFFFFF - 256 || a.kv_rows > 0x7FFFFFFF - 256)
     return invalid("q_rows and kv_rows must be below 2^31 - 256");
   if (a.documents < 0) return invalid("documents must not be negative");
-  if (!(a.scale > 0.f) || a.scale > 3.0e38f) return invalid("scale must be positive and finite");
-  if (!(a.softcap >= 0.f) || a.softcap > 3.0e38f) return invalid("softcap must be 0 (none) or positive and finite");
+  if (!(a.scale >= 1e-20f && a.scale <= 1e20f)) return invalid("scale must be from 1e-20 to 1e20");
+  if (a.softcap != 0.f && !(a.softcap >= 1e-15f && a.softcap <= 1e15f))
+    return invalid("softcap must be 0 (none) or from 1e-15 to 1e15");
   if (a.prefix && !a.causal) return invalid("a prefix needs causal");
   if (a.q_offsets) {
     if (!a.kv_offsets) return invalid("q_offsets and kv_offsets go together");

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   }
   const bool capped = p.cap > 0.f;
   const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
-  const float two_over_cap2 = capped ? 2.f * LOG2E * p.scale / p.cap : 0.f;
+  const float factor = capped ? p.scale / p.cap : 0.f;
   float slope2[2] = {0.f, 0.f};
   if (p.slopes) {
 #pragma unroll
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const long long key = key0 + n * 8 + (e & 1);
-        float z = capped ? capped_log2(s[n][e], two_over_cap2, cap2) : s[n][e] * scale2;
+        float z = capped ? capped_log2(s[n][e], factor, cap2) : s[n][e] * scale2;
         if (p.slopes) z = fmaf(-slope2[e >> 1], (float)llabs(key - iv.pos), z);
         z = key < iv.hi ? z : -INFINITY;
         s[n][e] = z;

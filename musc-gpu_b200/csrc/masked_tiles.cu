@@ -1,21 +1,29 @@
 // Masked attention of many query rows (masked.cuh has the operator): fused tcgen05 attention
-// over tiles of 256 query rows x 128 keys.
+// over tiles of 256 query rows x 64 keys.
 //
-// One CTA per (256 consecutive rows of the packed queries, head, split of the keys), 384
-// threads.  Its rows need not belong to one document: every row carries its own key interval,
-// and the CTA walks the union of its documents' intervals in tiles of 128 keys, so many
-// short documents share a tile and a long one pays nothing for the generality.
+// One CTA per (256 query rows, head, split of the keys), 384 threads.  Its rows need not belong
+// to one document: every row carries its own key interval, and the CTA walks the union of its
+// documents' intervals in tiles of 64 keys, so short documents share a row tile; long ones begin
+// their own (one that holds two long documents' rows walks both their keys: 4 x 1370 tokens of 16
+// heads take 100 us, 170 when tiles are cut from the packed rows).
 //   warps 0-3, 4-7  softmax of query rows 0-127 and 128-255 (the two halves), one thread
 //                   per row: S out of tensor memory, cap, bias, mask, running maximum and
-//                   sum in 32 bits, P rounded to 16 bits back into tensor memory over S;
+//                   sum in 32 bits, P rounded to 16 bits into tensor memory beside S;
 //   warp 8          TMA: Q once, K and V tiles through a ring;
 //   warps 9, 10     one thread for each half issues tcgen05.mma: S_h = Q_h K^T (128 x 64 x D,
 //                   both from shared memory) and O_h += P_h V (128 x D x 64, P from tensor memory);
 //   warp 11         zeroes the end of V's tiles that reach past their keys, and searches V.
-// While one half's softmax runs, the tensor cores work for the other: the exponentials
-// (16 a cycle and SM: 1024 cycles for 128 x 128) bound the kernel for D = 64 (256 cycles of
-// products at the tensor cores' rate) and for D = 128 (512).  O stays in tensor memory and is
-// rescaled only when a row's maximum has risen by more than 2^8 over the one in use.
+// While one half's softmax runs, the tensor cores work for the other.  For 64 keys the exponentials
+// of both halves take 1024 cycles (16 a cycle and SM), the products 700 for D = 64 and 1350 for D = 128
+// (S of 128 x 64 runs at two thirds of the rate of 128 x 128, whose S would leave no tensor memory
+// for P beside it).  Measured at 8192 tokens of 16 heads, no mask, bf16: D = 128 509 us (1080 TF/s, 0.64
+// of the measured 1693), D = 64 493 us (557 TF/s); four waves of CTAs for 3.46 waves of work.  The
+// special-function unit is 60 % busy, the tensor pipe 29 % (D = 64, ncu): the rest is the softmax warps'
+// own chain, two of them a scheduler.  Tried and dropped, with times at D = 64 or 128: tiles of 128 keys with P over
+// S (548 us), a maximum of every tile before its exponentials (no gain from leaving it out by itself, but
+// it frees registers), a share of the exponentials by polynomials (8 % slower: instructions
+// bound it as much), strict turns of the two halves' exponentials (no gain, and a half that is
+// tiles ahead of the other cannot wait for it), one issuing thread for both halves (596 us).
 //
 // A masked probability is zero, but zero times a NaN or infinite value is NaN.  Keys that no
 // row of the CTA sees (behind a document's last key) are zeroed in V's tile.  Tiles that some row
@@ -202,8 +210,7 @@ __device__ __forceinline__ void cap_scores(float2 (&s)[BKV / 2], float factor_, 
   for (int i = 0; i < BKV / 2; ++i) top = max3(top, fabsf(s[i].x), fabsf(s[i].y));
   const float x_max = top * factor;
   if (__all_sync(0xffffffffu, x_max <= 0.4f)) {
-    const float2 c0 = both(cap2 * 0.999999583f), c1 = both(cap2 * -0.333297253f), c2 = both(cap2 * 0.13250567f),
-                 c3 = both(cap2 * -0.0468257405f);
+    const float2 c0 = both(cap2 * TANH3[0]), c1 = both(cap2 * TANH3[1]), c2 = both(cap2 * TANH3[2]), c3 = both(cap2 * TANH3[3]);
 #pragma unroll
     for (int i = 0; i < BKV / 2; ++i) {
       const float2 x = mul2(s[i], both(factor)), t = mul2(x, x);
@@ -221,8 +228,8 @@ __device__ __forceinline__ void cap_scores(float2 (&s)[BKV / 2], float factor_, 
   } else {
 #pragma unroll
     for (int i = 0; i < BKV / 2; ++i) {
-      s[i].x = capped_log2(s[i].x, 2.f * LOG2E * factor, cap2);
-      s[i].y = capped_log2(s[i].y, 2.f * LOG2E * factor, cap2);
+      s[i].x = capped_log2(s[i].x, factor, cap2);
+      s[i].y = capped_log2(s[i].y, factor, cap2);
     }
   }
 }
@@ -282,7 +289,7 @@ __device__ __forceinline__ void rows_key_by_key(const Params& p, const int2* seg
         float dot = 0.f;
         for (int i = 0; i < N; ++i) dot = fmaf(qf[i], widen<FP16>(k[i]), dot);
         dot = warp_sum(dot);
-        float z = p.cap > 0.f ? capped_log2(dot, 2.f * LOG2E * p.scale / p.cap, p.cap * LOG2E) : dot * p.scale * LOG2E;
+        float z = p.cap > 0.f ? capped_log2(dot, p.scale / p.cap, p.cap * LOG2E) : dot * p.scale * LOG2E;
         if (p.slopes) z = fmaf(-slope2, fabsf((float)(key - pos)), z);
         const float m_new = fmaxf(m, z);
         const float a = m == -INFINITY ? 0.f : ex2(m - m_new);

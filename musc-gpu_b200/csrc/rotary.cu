@@ -231,6 +231,9 @@ extern "C" int musc_b200_rotary(const void* q, const void* k, void* q_out, void*
   if (tokens == 0) return MUSC_B200_OK;
   if (!q || !q_out || !positions || !frequencies || !axis || (kv_heads > 0 && (!k || !k_out)))
     return fail(MUSC_B200_ERR_INVALID, "rotary: null pointer");
+  for (const void* ptr : {positions, (const void*)frequencies, (const void*)axis})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4 != 0)
+      return fail(MUSC_B200_ERR_INVALID, "rotary: positions, frequencies and axis must be aligned to 4 bytes");
   const long long widths[2] = {(long long)heads * head_dim, (long long)kv_heads * head_dim};
   const int size = dtype == MUSC_B200_F32 ? 4 : 2;
   Params p;

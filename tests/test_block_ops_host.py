@@ -26,6 +26,7 @@ def _attention_args(**changes):
     (dict(kv_heads=0), 'multiple of kv_heads'), (dict(q_rows=-1), 'q_rows'), (dict(kv_rows=1 << 31), 'q_rows'),
     (dict(documents=-1), 'documents'), (dict(scale=0.0), 'scale'), (dict(scale=float('nan')), 'scale'),
     (dict(scale=float('inf')), 'scale'), (dict(softcap=-1.0), 'softcap'), (dict(softcap=float('nan')), 'softcap'),
+    (dict(softcap=1e-20), 'softcap'), (dict(softcap=1e20), 'softcap'), (dict(scale=-1.0), 'scale'),
     (dict(causal=0, prefix=1 << 20), 'prefix'), (dict(kv_offsets=None), 'go together'),
     (dict(q_offsets=None), 'go together'),
     (dict(q_offsets=None, kv_offsets=None, q_len=4, kv_len=10, kv_pitch=10), 'make q_rows'),
@@ -77,7 +78,7 @@ def _rotary(**changes):
     (dict(dtype=_lib.E4M3), 'dtype'), (dict(tokens=-1), 'tokens'), (dict(heads=0), 'heads'), (dict(axes=0), 'axes'),
     (dict(pairs=33), 'pairs'), (dict(pairs=0), 'pairs'), (dict(head_dim=514), 'head_dim'), (dict(q=None), 'null'),
     (dict(k_out=None), 'null'), (dict(positions=None), 'null'), (dict(q_stride=255), 'strides'),
-    (dict(q=(1 << 20) + 1), 'aligned'),
+    (dict(q=(1 << 20) + 1), 'aligned'), (dict(positions=(5 << 20) + 2), 'aligned'), (dict(axis=(7 << 20) + 1), 'aligned'),
     (dict(q_out=(1 << 20) + 16), 'overlap'),                       # shifted by half a row
     (dict(q_out=2 << 20), 'overlap'),                              # onto the other input
     (dict(k_out=3 << 20), 'overlap'),                              # two outputs in one place
@@ -112,6 +113,7 @@ def _norm(**changes):
     (dict(x=None), 'null'), (dict(scales=None), 'null'), (dict(weight=None), 'null'), (dict(x_stride=999), 'strides'),
     (dict(delta_stride=5), 'strides'), (dict(x=(1 << 20) + 2), 'aligned'), (dict(out=(1 << 20) + 16), 'overlap'),
     (dict(out=(2 << 20) + 16), 'overlap'), (dict(delta=(1 << 20) + 4000), 'overlap'),
+    (dict(out=(3 << 20) + 16), 'overlap'), (dict(weight=(1 << 20) + 16), 'overlap'),
     (dict(scales=(1 << 20) + 8), 'overlap'), (dict(scales=(4 << 20) + 8), 'overlap'),
 ])
 def test_norm_contract(changes, message):

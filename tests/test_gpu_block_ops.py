@@ -296,6 +296,27 @@ def test_attention_long_axis(cuda_device, n_q, n_k, dtype):
     _assert_close(got, *_reference(q, k, v, 2, 1, [0, n_q], [0, n_k]))
 
 
+@pytest.mark.parametrize('n_q', [2, 200])
+@pytest.mark.parametrize('softcap', [0.01, 3.0, 1e4, 1e7])
+def test_attention_cap_far_from_the_scores(cuda_device, n_q, softcap):
+    """Caps far below the scores (all of them at the cap) and far above: tanh(z / cap) * cap keeps the relative
+    accuracy of 32 bits for small z / cap too, so the bound is the uncapped one's and 2^-20 of min(|z|, cap)."""
+    from musc_b200 import ops
+    q, k, v = _random_qkv(cuda_device, n_q, 700, 2, 1, 64, torch.float16, 31, False)
+    q = q * 3
+    offsets = dict(offsets=_i32([0, n_q], cuda_device), kv_offsets=_i32([0, 700], cuda_device))
+    got = ops.attention_masked(q, k, v, 2, 1, softcap=softcap, **offsets)
+    want, _ = _reference(q, k, v, 2, 1, [0, n_q], [0, 700], softcap=softcap)
+    _, tol = _reference(q, k, v, 2, 1, [0, n_q], [0, 700])
+    mean = torch.cat([_reference(q[:, h * 64:(h + 1) * 64], k, v.abs(), 1, 1, [0, n_q], [0, 700], softcap=softcap)[0]
+                      for h in range(2)], 1)
+    size = float((q.double().view(-1, 64) @ k.double().T / 8).abs().max())
+    # the rounding of P and of the result, on the capped scores' own average
+    tol = torch.maximum(tol, 2.0 ** -11 * (mean + want.abs()) * (1 + 2.0 ** -6) + 2.0 ** -24)
+    tol = tol + 2 * mean * ((64 + 8) * 2.0 ** -24 * 8 * size + 2.0 ** -18 + min(size, softcap) * 2.0 ** -20)
+    _assert_close(got, want, tol)
+
+
 def test_attention_captured_and_on_other_streams(cuda_device):
     """Replays of two graphs and eager calls on two streams give the eager result bit for bit."""
     from musc_b200 import ops
