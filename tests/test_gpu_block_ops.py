@@ -296,6 +296,88 @@ def test_attention_long_axis(cuda_device, n_q, n_k, dtype):
     _assert_close(got, *_reference(q, k, v, 2, 1, [0, n_q], [0, n_k]))
 
 
+def _lengths(kind, seed):
+    g = torch.Generator().manual_seed(seed)
+    if kind == 'middling':      # 60 documents, some longer than a row tile, some empty
+        n = torch.randint(0, 160, (60,), generator=g)
+        n[::9] += 300
+        n[5] = n[6] = 0
+    elif kind == 'tiny':        # more documents than are looked up in shared memory
+        n = torch.randint(8, 28, (1100,), generator=g)
+    elif kind == 'one_of_many': # one long document among short ones
+        n = torch.randint(1, 90, (33,), generator=g)
+        n[20] = 1500
+    else:                       # long ones, ending at and beside tile borders
+        n = torch.tensor([256, 255, 257, 512, 1, 64, 65, 700])
+    return n.tolist()
+
+
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('kind,d', [('middling', 64), ('tiny', 64), ('one_of_many', 128), ('long', 128)])
+def test_attention_many_documents(cuda_device, kind, d, causal):
+    """Row tiles of many documents, packed rows before the first and behind the last one left alone."""
+    from musc_b200 import ops
+    lens = _lengths(kind, 40)
+    off = [13 + o for o in _starts(lens)]
+    q, k, v = _random_qkv(cuda_device, off[-1] + 30, off[-1] + 30, 2, 1, d, torch.bfloat16, 41, True)
+    out = torch.full_like(q, 3.0)
+    ops.attention_masked(q, k, v, 2, 1, offsets=_i32(off, cuda_device), causal=causal, out=out)
+    assert bool((out[:13] == 3).all()) and bool((out[off[-1]:] == 3).all())
+    want, tol = _reference(q, k, v, 2, 1, off, off, causal=causal)
+    _assert_close(out[13:off[-1]], want[13:off[-1]], tol[13:off[-1]])
+
+
+@pytest.mark.parametrize('length', [17, 100, 256, 300, 515])
+def test_attention_batches_of_one_length(cuda_device, length):
+    from musc_b200 import ops
+    q, k, v = _random_qkv(cuda_device, 5 * length, 5 * length, 4, 2, 64, torch.float16, 42, True)
+    view = lambda t: t.unflatten(0, (5, length))
+    got = ops.attention_masked(view(q), view(k), view(v), 4, 2, causal=True, softcap=20.0)
+    off = _starts([length] * 5)
+    _assert_close(got.flatten(0, 1), *_reference(q, k, v, 4, 2, off, off, causal=True, softcap=20.0))
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('n_q', [4, 150])
+@pytest.mark.parametrize('poison', [0.0, math.nan])
+def test_attention_split_documents(cuda_device, n_q, poison, d):
+    """Several documents of few rows over long keys: both kernels split the keys; a NaN in a value that only the
+    last rows see stays with them."""
+    from musc_b200 import ops
+    docs, keys = 2, [9001, 5003]
+    q, k, v = _random_qkv(cuda_device, docs * n_q, sum(keys), 2, 1, d, torch.float16, 43, False)
+    q_off, k_off = _starts([n_q] * docs), _starts(keys)
+    prefix = [4000, 5003]
+    clean = v.clone()
+    v[k_off[1] - 2, 5] = poison                    # the last but one key of the first document
+    got = ops.attention_masked(q, k, v, 2, 1, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               causal=True, prefix=_i32(prefix, cuda_device))
+    want, tol = _reference(q, k, clean if math.isnan(poison) else v, 2, 1, q_off, k_off, causal=True, prefix=prefix)
+    rows = [r for r in range(docs * n_q) if not (math.isnan(poison) and n_q - 2 <= r < n_q)]
+    _assert_close(got[rows], want[rows], tol[rows])
+    if math.isnan(poison):
+        assert torch.isnan(got[n_q - 2:n_q, [5, 5 + d]]).all()
+        others = [c for c in range(2 * d) if c % d != 5]
+        _assert_close(got[n_q - 2:n_q][:, others], want[n_q - 2:n_q][:, others], tol[n_q - 2:n_q][:, others])
+
+
+@pytest.mark.parametrize('n', [20, 900])
+def test_attention_disordered_offsets_stay_inside(cuda_device, n):
+    """Offsets that fall, repeat or leave the tensors: results are undefined, accesses are not."""
+    from musc_b200 import ops
+    q, k, v = _random_qkv(cuda_device, n, n, 2, 1, 64, torch.float16, 44, True)
+    top = (1 << 31) - 1
+    for q_off, k_off in (([0, n, 5, n], [0, 3, 2, n]), ([-7, 3, n // 2, top], [top, 0, -top, 9]), ([0, top, 0, n], [5, 5, 5, 5]),
+                         ([n, n - 1, 2, 0], [0, n, 0, n]), ([-top - 1, top, -5, top], [-1, -1, top, top])):
+        for causal in (False, True):
+            ops.attention_masked(q, k, v, 2, 1, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                                 kv_lengths=_i32([top, -3, 4], cuda_device), causal=causal)
+    torch.cuda.synchronize()
+    ops.check_device_error(cuda_device)
+    got = ops.attention_masked(q, k, v, 2, 1, offsets=_i32([0, n], cuda_device))
+    _assert_close(got, *_reference(q, k, v, 2, 1, [0, n], [0, n]))
+
+
 @pytest.mark.parametrize('n_q', [2, 200])
 @pytest.mark.parametrize('softcap', [0.01, 3.0, 1e4, 1e7])
 def test_attention_cap_far_from_the_scores(cuda_device, n_q, softcap):
