@@ -2,6 +2,7 @@
 // kernel and of the splits, and the kernel that joins the splits' partial sums.
 #include "masked.cuh"
 
+#include <algorithm>
 #include <string>
 
 namespace musc {
@@ -73,7 +74,7 @@ namespace {
 
 struct Plan {
   bool tiles = false;
-  int splits = 1;
+  int splits = 1, block_rows = 1;
   size_t ml_offset = 0, bytes = 0;
 };
 
@@ -86,13 +87,17 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   Plan plan;
   const long long rows = a.q_rows * a.heads;
   const int group = a.heads / a.kv_heads;
-  // A CTA of the tile kernel takes 256 rows of one head, one of the row kernel one row of all
-  // heads of a key head (up to 16), reading its keys again for every row.
+  // A CTA of the tile kernel takes 256 rows of one head, one of the row kernel up to 16 rows x heads of
+  // one document and key head.
   plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
   if (plan.tiles)
     plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a), a.causal != 0);
-  else
-    plan.splits = rows_splits(a.q_rows * a.kv_heads * ((group + 15) / 16), mean_keys(a), a.q_rows <= a.documents);
+  else {
+    plan.block_rows = rows_together(group, a.q_rows > a.documents);
+    const long long used = std::min<long long>(plan.block_rows, (a.q_rows + a.documents - 1) / a.documents);
+    plan.splits = rows_splits((a.q_rows + used - 1) / used * a.kv_heads * ((group + 15) / 16), mean_keys(a),
+                              a.q_rows <= a.documents * used);
+  }
   if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {
     plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;
     plan.bytes = plan.ml_offset + (size_t)plan.splits * rows * sizeof(float2);
@@ -189,6 +194,12 @@ extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args*
   p.heads = a.heads, p.kv_heads = a.kv_heads, p.group = a.heads / a.kv_heads;
   p.causal = a.causal, p.scale = a.scale, p.cap = a.softcap;
   p.splits = plan.splits;
+  // A document's blocks of rows begin at its first row.  Packed, document d's are counted from
+  // q_offsets[d] / block_rows + d on, which leaves room for the last one of every document.
+  p.block_rows = plan.block_rows;
+  p.row_blocks = p.block_rows == 1 ? a.q_rows
+                 : a.q_offsets     ? a.q_rows / p.block_rows + a.documents
+                                   : a.documents * ((a.q_len + p.block_rows - 1) / p.block_rows);
   p.part = static_cast<float*>(a.workspace);
   p.part_ml = plan.bytes ? reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + plan.ml_offset) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

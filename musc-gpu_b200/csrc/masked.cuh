@@ -45,13 +45,23 @@ struct Params {
   int* err;
   // Tile kernel: grid of row tiles, and whether documents begin their own (masked_tiles.cu).
   int row_tiles, aligned;
+  // Row kernel: rows of a document that a CTA takes, and the number of such blocks of rows that are looked at.
+  int block_rows;
+  long long row_blocks;
 };
 
 // Keys [lo, hi) of the packed keys that a row sees, and the key its own position falls on.
 // lo is the first key of the row's document.  Whatever the offsets hold, 0 <= lo <= hi <= kv_rows.
+// Also the document's keys, those that every row of it sees, and the rows from this one to its last.
 struct Interval {
-  long long lo, hi, pos;
+  long long lo, hi, pos, keys, least, rows_left;
 };
+
+// End of the keys that the row `after` rows behind an interval's own sees, in the same document.
+__device__ __forceinline__ long long interval_end(const Params& p, const Interval& iv, int after) {
+  if (!p.causal) return iv.lo + iv.keys;
+  return iv.lo + min(max(max(iv.pos + after + 1 - iv.lo, iv.least), 0LL), iv.keys);
+}
 
 // Document of a row: the last one that begins at or before it.  -1: the row belongs to none.
 __device__ __forceinline__ int find_document(const Params& p, long long row) {
@@ -64,18 +74,6 @@ __device__ __forceinline__ int find_document(const Params& p, long long row) {
     else hi = mid;
   }
   return lo;
-}
-
-// The same by a converged warp, in one load's time for up to 1024 documents: the lanes count the
-// documents that begin at or before the row.
-__device__ __forceinline__ int find_document_warp(const Params& p, long long row) {
-  if (!p.q_offsets || p.documents > 1024) return find_document(p, row);
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-#pragma unroll 8
-  for (int i = lane; i <= p.documents; i += 32) before += __ldg(p.q_offsets + i) <= row ? 1 : 0;
-  before = __reduce_add_sync(0xffffffffu, before);
-  return before > 0 && before <= p.documents ? before - 1 : -1;
 }
 
 __device__ __forceinline__ Interval row_interval(const Params& p, int doc, long long row) {
@@ -95,13 +93,10 @@ __device__ __forceinline__ Interval row_interval(const Params& p, int doc, long 
   Interval r;
   r.lo = k0;
   r.pos = k0 + (row - q0) + (nk - nq);
-  long long seen = nk;
-  if (p.causal) {
-    seen = r.pos + 1 - k0;
-    if (p.prefix) seen = max(seen, (long long)__ldg(p.prefix + doc));
-    seen = min(max(seen, 0LL), nk);
-  }
-  r.hi = k0 + seen;
+  r.keys = nk;
+  r.least = p.causal && p.prefix ? __ldg(p.prefix + doc) : 0;
+  r.rows_left = q0 + nq - row;
+  r.hi = interval_end(p, r, 0);
   return r;
 }
 
@@ -138,6 +133,36 @@ __device__ __forceinline__ float capped_log2(float s, float factor, float cap2) 
 template <bool FP16>
 constexpr float RAISE = FP16 ? 6.f : 0.f;
 
+template <bool FP16>
+__device__ __forceinline__ float widen(uint16_t v) {
+  return FP16 ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
+}
+
+// A row and head's sums over keys [first, end) by a warp, key by key: lanes hold D / 32 dimensions of q and
+// of the sums.  The slow form, for rows beside values that are not finite and that they do not see.
+template <int D, bool FP16>
+__device__ __forceinline__ void attend_keys(const Params& p, const float (&q)[D / 32], int kv_head, float slope2, long long pos,
+                                            long long first, long long end, float (&acc)[D / 32], float& m, float& l) {
+  constexpr int N = D / 32;
+  const int lane = threadIdx.x & 31;
+  for (long long key = first; key < end; ++key) {
+    const uint16_t* k = static_cast<const uint16_t*>(p.k) + key * p.k_stride + kv_head * D + lane * N;
+    const uint16_t* v = static_cast<const uint16_t*>(p.v) + key * p.v_stride + kv_head * D + lane * N;
+    float dot = 0.f;
+    for (int i = 0; i < N; ++i) dot = fmaf(q[i], widen<FP16>(k[i]), dot);
+    dot = warp_sum(dot);
+    float z = p.cap > 0.f ? capped_log2(dot, p.scale / p.cap, p.cap * LOG2E) : dot * p.scale * LOG2E;
+    if (p.slopes) z = fmaf(-slope2, (float)llabs(key - pos), z);
+    const float m_new = fmaxf(m, z);
+    const float a = m == -INFINITY ? 0.f : ex2(m - m_new);
+    m = m_new;
+    // a key whose score is -inf adds nothing, NaN scores add NaN
+    const float e = z == -INFINITY ? 0.f : ex2(z - m);
+    l = fmaf(l, a, e);
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(e, widen<FP16>(v[i]), acc[i] * a);
+  }
+}
+
 // A split's partial result of a row and head: its reference maximum and its sum.  The maximum of a
 // row that sees keys is finite even where it met none of them; (-inf, 0) says that it sees no key.
 __device__ __forceinline__ float2 partial_ml(float m, float l, bool any_key) {
@@ -160,7 +185,8 @@ __device__ __forceinline__ float inverse_sum(float l, bool any_key) {
 // when a document has about `keys` keys.
 constexpr int MAX_CLUSTER = 8;  // up to so many splits the row kernel joins by itself, without a workspace
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
-int rows_splits(long long units, long long keys, bool single);  // single: one row for each document
+int rows_together(int group, bool several);  // several: rows a document
+int rows_splits(long long units, long long keys, bool single);  // single: documents of one block of rows each
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int tiles_splits(long long units, long long keys, bool causal);
 bool tiles_aligned(const Params& p);

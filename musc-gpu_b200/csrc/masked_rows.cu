@@ -1,9 +1,9 @@
 // Masked attention of few query rows against many keys (masked.cuh has the operator): one
-// CTA per query row, key head and split of the row's keys.
+// CTA per query row (or a few of one document), key head and split of the keys.
 //
-// A row's keys and values are read once for all query heads of their group, and nothing else
-// is large: memory bounds it.  The group's heads are the 16 rows of the tensor core's
-// m16n8k16 products (a larger group takes several CTAs): S = Q K^T over 16 keys and the head
+// Keys and values are read once for all query heads of their group, and nothing else
+// is large: memory bounds it.  The group's heads, for as many consecutive rows of a document as fit, are
+// the 16 rows of the tensor core's m16n8k16 products (a larger group takes several CTAs): S = Q K^T over 16 keys and the head
 // dimension, then O += P V, at 2 x 16 x 16 x D operations per 64 D bytes far below what the
 // tensor cores give.  Each of the CTA's warps takes every WARPS-th run of 16 keys through a
 // ring of its own that cp.async fills STAGES runs ahead, so no barrier stands between a
@@ -24,7 +24,7 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int KEYS = 16;    // keys of a warp's step
 constexpr int STAGES = 2;   // steps in flight per warp: WARPS x STAGES x 64 D bytes a CTA
-constexpr int HEADS = 16;   // query heads of a CTA
+constexpr int HEADS = 16;   // rows of the products: rows x query heads of a CTA
 // Splits.  Three waves of what is resident (148 SMs x 3 CTAs) even out documents of differing lengths:
 // 32 tokens over 8192 keys in 116 us, 132 with one wave.  Where several rows of a document read its keys
 // from L2, one wave keeps them together: 2 rows over 6390 keys in 32 us, 38 with three.
@@ -100,8 +100,43 @@ __device__ __forceinline__ void store_eight(const Params& p, long long row, int 
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.out_stride + column) = packed;
 }
 
-template <int D, bool FP16, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
+// Document and first row of a block of rows, by a converged warp; -1: it holds no row.  The lanes count the
+// documents whose blocks begin at or before this one.
+template <bool SEVERAL>
+__device__ __forceinline__ int find_block(const Params& p, long long block, long long& row) {
+  const int size = SEVERAL ? p.block_rows : 1;
+  if (!p.q_offsets) {
+    const int per_doc = (int)((p.q_len + size - 1) / size), doc = (int)(block / per_doc);
+    row = doc * p.q_len + (block - (long long)doc * per_doc) * size;
+    return doc;
+  }
+  const auto begin = [&](int d) {
+    const int first = __ldg(p.q_offsets + d);
+    return SEVERAL ? (long long)(first / size) + d : (long long)first;
+  };
+  int doc;  // the last document that begins at or before the block
+  if (p.documents > 1024) {
+    int lo = -1, hi = p.documents;  // begin(lo) <= block < begin(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (begin(mid) <= block) lo = mid;
+      else hi = mid;
+    }
+    doc = lo;
+  } else {  // one load's time
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+#pragma unroll 8
+    for (int i = lane; i < p.documents; i += 32) before += begin(i) <= block ? 1 : 0;
+    doc = (int)__reduce_add_sync(0xffffffffu, before) - 1;
+  }
+  if (doc < 0) return -1;
+  row = SEVERAL ? __ldg(p.q_offsets + doc) + (block - begin(doc)) * size : block;
+  return row >= 0 && row < min((long long)__ldg(p.q_offsets + doc + 1), p.q_rows) ? doc : -1;
+}
+
+template <int D, bool FP16, bool CLUSTER, bool SEVERAL>
+__global__ void __launch_bounds__(THREADS, D == 64 ? 4 : 3) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
   constexpr int CHUNKS = D / 8;  // 16-byte chunks of a key
@@ -109,30 +144,35 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   // Neighbouring CTAs take neighbouring rows: those of one document share its keys in L2.
   long long unit = blockIdx.x / p.splits;
   const int split = (int)(blockIdx.x - unit * p.splits);
-  const long long row = unit % p.q_rows;
-  unit /= p.q_rows;
+  const long long row_block = unit % p.row_blocks;
+  unit /= p.row_blocks;
   const int kv_head = (int)(unit % p.kv_heads), block = (int)(unit / p.kv_heads);
   const int head0 = kv_head * p.group + block * HEADS;
   const int n_heads = min(HEADS, p.group - block * HEADS);
-  const int doc = find_document_warp(p, row);
+  long long row;
+  const int doc = find_block<SEVERAL>(p, row_block, row);
   if (doc < 0) return;  // uniform over the CTA and its cluster
   const Interval iv = row_interval(p, doc, row);
-  // This split's share of the interval, in whole steps.
-  const long long steps = (iv.hi - iv.lo + KEYS - 1) / KEYS;
-  const long long first = steps * split / p.splits, last = steps * (split + 1) / p.splits;
+  const int n_tokens = SEVERAL ? (int)min(min((long long)p.block_rows, iv.rows_left), p.q_rows - row) : 1;
+  const int n_rows = n_tokens * n_heads;  // row r: token r / n_heads, head r % n_heads
+  // Keys that all of them see, in whole steps; then those that only the later ones do (fewer than a step).
+  const int lo = (int)iv.lo, common = (int)iv.hi, end = (int)interval_end(p, iv, n_tokens - 1);
+  const int main_steps = (common - lo + KEYS - 1) / KEYS, steps = main_steps + (SEVERAL && end > common ? 1 : 0);
+  const int first = (int)((long long)steps * split / p.splits), last = (int)((long long)steps * (split + 1) / p.splits);
+  const auto step_key = [&](int step) { return !SEVERAL || step < main_steps ? lo + step * KEYS : common; };
   const uint16_t* k_base = static_cast<const uint16_t*>(p.k) + kv_head * D;
   const uint16_t* v_base = static_cast<const uint16_t*>(p.v) + kv_head * D;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sm.ring[warp][0][0][0]));
   constexpr uint32_t HALF = KEYS * D * 2;  // bytes of a step's K (or V)
   // The warp's i-th step is step first + warp + i * WARPS.
-  const auto load = [&](long long step, int stage) {
+  const auto load = [&](int step, int stage) {
     if (step < last) {
-      const long long key0 = iv.lo + step * KEYS;
+      const int key0 = step_key(step), stop = !SEVERAL || step < main_steps ? common : end;
 #pragma unroll
       for (int i = 0; i < KEYS * CHUNKS / 32; ++i) {
         const int c = i * 32 + lane, key = c / CHUNKS, chunk = c % CHUNKS;
-        const bool take = key0 + key < iv.hi;
-        const long long at = take ? key0 + key : iv.lo;
+        const bool take = key0 + key < stop;
+        const long long at = take ? key0 + key : lo;
         const uint32_t dst = ring + stage * 2 * HALF + key * (D * 2) + ((chunk ^ (key & 7)) << 4);
         cp_async16(dst, k_base + at * p.k_stride + chunk * 8, take);
         cp_async16(dst + HALF, v_base + at * p.v_stride + chunk * 8, take);
@@ -143,39 +183,43 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load(first + warp + s * WARPS, s);
 
-  // Query heads as the A operand: row r = head0 + r, zeros past the group.
-  uint32_t qa[D / 16][4];
-  {
-    const uint16_t* q = static_cast<const uint16_t*>(p.q) + row * p.q_stride + (long long)head0 * D;
-    const int r = lane >> 2, c = (lane & 3) * 2;
+  // Queries as the A operand, zeros past the last row.  This lane's rows are lane / 4 and lane / 4 + 8.
+  int token[2], head[2];
+  const uint16_t* q_row[2];
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) {
-      const uint16_t* a = q + r * D + t * 16 + c;
-      const uint16_t* b = a + 8 * D;
-      qa[t][0] = r < n_heads ? *reinterpret_cast<const uint32_t*>(a) : 0u;
-      qa[t][1] = r + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(b) : 0u;
-      qa[t][2] = r < n_heads ? *reinterpret_cast<const uint32_t*>(a + 8) : 0u;
-      qa[t][3] = r + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(b + 8) : 0u;
-    }
+  for (int h = 0; h < 2; ++h) {
+    const int r = (lane >> 2) + 8 * h;
+    token[h] = SEVERAL ? r / n_heads : 0;
+    head[h] = r - token[h] * n_heads;
+    q_row[h] = r < n_rows ? static_cast<const uint16_t*>(p.q) + (row + token[h]) * p.q_stride + (long long)(head0 + head[h]) * D
+                          : nullptr;
   }
+  uint32_t qa[D / 16][4];
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t* at = q_row[i & 1];
+      qa[t][i] = at ? *reinterpret_cast<const uint32_t*>(at + t * 16 + (lane & 3) * 2 + (i >> 1) * 8) : 0u;
+    }
   const bool capped = p.cap > 0.f;
   const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E;
   const float factor = capped ? p.scale / p.cap : 0.f;
   float slope2[2] = {0.f, 0.f};
   if (p.slopes) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = (lane >> 2) + 8 * h;
-      if (r < n_heads) slope2[h] = __ldg(p.slopes + head0 + r) * LOG2E;
-    }
+    for (int h = 0; h < 2; ++h)
+      if (q_row[h]) slope2[h] = __ldg(p.slopes + head0 + head[h]) * LOG2E;
   }
+  const int own_end[2] = {(int)interval_end(p, iv, token[0]), (int)interval_end(p, iv, token[1])};
 
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // rows lane / 4 and lane / 4 + 8; l of this lane's keys
   int stage = 0;
-  for (long long step = first + warp; step < last; step += WARPS) {
+  bool redo = false;
+  for (int step = first + warp; step < last; step += WARPS) {
     load(step + (STAGES - 1) * WARPS, (stage + STAGES - 1) % STAGES);
     cp_async_wait<STAGES - 1>();
     __syncwarp();
@@ -193,16 +237,18 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       mma16816<FP16>(s[1], qa[t], b[1], b[3]);
     }
     // Scores of keys key0 + {0, 1} and key0 + 8 + {0, 1}, key0 of this lane.
-    const long long key0 = iv.lo + step * KEYS + (lane & 3) * 2;
+    const int key0 = step_key(step) + (lane & 3) * 2;
+    const bool tail = SEVERAL && step >= main_steps;
+    const int stop[2] = {tail ? own_end[0] : common, tail ? own_end[1] : common};
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const long long key = key0 + n * 8 + (e & 1);
+        const int key = key0 + n * 8 + (e & 1);
         float z = capped ? capped_log2(s[n][e], factor, cap2) : s[n][e] * scale2;
-        if (p.slopes) z = fmaf(-slope2[e >> 1], (float)llabs(key - iv.pos), z);
-        z = key < iv.hi ? z : -INFINITY;
+        if (p.slopes) z = fmaf(-slope2[e >> 1], (float)llabs(key - iv.pos - token[e >> 1]), z);
+        z = key < stop[e >> 1] ? z : -INFINITY;
         s[n][e] = z;
         top[e >> 1] = fmaxf(top[e >> 1], z);
       }
@@ -241,6 +287,11 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       const int key = (lane & 7) + ((lane >> 3) & 1) * 8, chunk = t * 2 + (lane >> 4);
       uint32_t b[4];
       ldmatrix4_trans(b, vt + key * (D * 2) + ((chunk ^ (key & 7)) << 4));
+      if (tail) {  // values that are not finite, beside rows that do not see them: exponent bits all ones
+        constexpr uint32_t EXP = FP16 ? 0x7C007C00u : 0x7F807F80u, UNIT = FP16 ? 0x04000400u : 0x00800080u;
+        if ((((b[0] & EXP) + UNIT) | ((b[1] & EXP) + UNIT) | ((b[2] & EXP) + UNIT) | ((b[3] & EXP) + UNIT)) & 0x80008000u)
+          redo = true;
+      }
       mma16816<FP16>(o[2 * t], pa, b[0], b[1]);
       mma16816<FP16>(o[2 * t + 1], pa, b[2], b[3]);
     }
@@ -248,7 +299,9 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
     stage = (stage + 1) % STAGES;
   }
   cp_async_wait<0>();
-  __syncthreads();  // the rings' memory becomes the warps' sums
+  // The rings' memory becomes the warps' sums.
+  if (SEVERAL) redo = __syncthreads_or(redo);
+  else __syncthreads();
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -260,8 +313,33 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       *reinterpret_cast<float2*>(&sm.o[warp][r][n * 8 + (lane & 3) * 2]) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < n_heads * (D / 8); e += THREADS) {
+  if (redo) {
+    // The rows again, each by a warp, over the keys of this split that it sees.
+    constexpr int N = D / 32;
+    for (int r = warp; r < n_rows; r += WARPS) {
+      const int t = SEVERAL ? r / n_heads : 0, h = head0 + r - t * n_heads;
+      const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row + t) * p.q_stride + (long long)h * D + lane * N;
+      float qf[N], acc[N], m_row = -INFINITY, l_row = 0.f;
+      for (int i = 0; i < N; ++i) qf[i] = widen<FP16>(q[i]), acc[i] = 0.f;
+      const float slope = p.slopes ? __ldg(p.slopes + h) * LOG2E : 0.f;
+      const int main_last = min(last, main_steps);
+      const long long own = interval_end(p, iv, t);
+      if (first < main_last)
+        attend_keys<D, FP16>(p, qf, kv_head, slope, iv.pos + t, step_key(first), min(step_key(main_last - 1) + KEYS, common), acc,
+                             m_row, l_row);
+      if (last > main_steps)
+        attend_keys<D, FP16>(p, qf, kv_head, slope, iv.pos + t, step_key(max(first, main_steps)), own, acc, m_row, l_row);
+      for (int w = 0; w < WARPS; ++w) {  // in the place of the first warp's sums; those carry RAISE
+        for (int i = 0; i < N; ++i) sm.o[w][r][lane * N + i] = w == 0 ? acc[i] : 0.f;
+        if (lane == 0) sm.ml[w][r][0] = w == 0 ? m_row + RAISE<FP16> : -INFINITY, sm.ml[w][r][1] = w == 0 ? l_row : 0.f;
+      }
+    }
+    __syncthreads();
+  }
+  for (int e = threadIdx.x; e < n_rows * (D / 8); e += THREADS) {
     const int r = e / (D / 8), d = e % (D / 8) * 8;
+    const int t = SEVERAL ? r / n_heads : 0, h = head0 + r - t * n_heads;
+    const bool any_key = interval_end(p, iv, t) > lo;
     float common = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) common = fmaxf(common, sm.ml[w][r][0]);
@@ -276,14 +354,14 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
       for (int i = 0; i < 8; ++i) acc[i] = fmaf(f, sm.o[w][r][d + i], acc[i]);
     }
     if (CLUSTER) {
-      if (d == 0) sm.sums_ml[r] = partial_ml(common, total, iv.hi > iv.lo);
+      if (d == 0) sm.sums_ml[r] = partial_ml(common, total, any_key);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sm.sums[r][d + i] = acc[i];
     } else if (p.splits == 1) {
-      store_eight<FP16>(p, row, (head0 + r) * D + d, acc, inverse_sum(total, iv.hi > iv.lo));
+      store_eight<FP16>(p, row + t, h * D + d, acc, inverse_sum(total, any_key));
     } else {
-      const long long at = (split * p.q_rows + row) * p.heads + head0 + r;
-      if (d == 0) p.part_ml[at] = partial_ml(common, total, iv.hi > iv.lo);
+      const long long at = (split * p.q_rows + row + t) * p.heads + h;
+      if (d == 0) p.part_ml[at] = partial_ml(common, total, any_key);
       if (total != 0.f) {
         *reinterpret_cast<float4*>(p.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         *reinterpret_cast<float4*>(p.part + at * D + d + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
@@ -293,8 +371,8 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
   if (CLUSTER) {
     // Every CTA of the cluster joins its share of the heads' dimensions, eight at a time.
     tc::cluster_sync();
-    for (int e = split * THREADS + threadIdx.x; e < n_heads * (D / 8); e += p.splits * THREADS) {
-      const int r = e / (D / 8), d = e % (D / 8) * 8;
+    for (int e = split * THREADS + threadIdx.x; e < n_rows * (D / 8); e += p.splits * THREADS) {
+      const int r = e / (D / 8), d = e % (D / 8) * 8, t = SEVERAL ? r / n_heads : 0;
       float2 ml[MAX_CLUSTER];
       float common = -INFINITY, total = 0.f, acc[8];
 #pragma unroll
@@ -316,15 +394,15 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(const Params p) {
           acc[2 * i] = fmaf(f, o.x, acc[2 * i]), acc[2 * i + 1] = fmaf(f, o.y, acc[2 * i + 1]);
         }
       }
-      store_eight<FP16>(p, row, (head0 + r) * D + d, acc, inverse_sum(total, common != -INFINITY));
+      store_eight<FP16>(p, row + t, (head0 + r - t * n_heads) * D + d, acc, inverse_sum(total, common != -INFINITY));
     }
     tc::cluster_sync();  // no CTA leaves while another reads its sums
   }
 }
 
-template <int D, bool FP16, bool CLUSTER>
+template <int D, bool FP16, bool CLUSTER, bool SEVERAL>
 int launch_as(const Params& p, long long grid, cudaStream_t s) {
-  constexpr auto kernel = rows_kernel<D, FP16, CLUSTER>;
+  constexpr auto kernel = rows_kernel<D, FP16, CLUSTER, SEVERAL>;
   MUSC_TRY(opt_in_smem<kernel>(sizeof(Smem<D>)));
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)grid);
@@ -343,13 +421,17 @@ int launch_as(const Params& p, long long grid, cudaStream_t s) {
 
 template <int D, bool FP16>
 int launch(const Params& p, cudaStream_t s) {
-  const long long grid = p.q_rows * p.kv_heads * ((p.group + HEADS - 1) / HEADS) * p.splits;
+  const long long grid = p.row_blocks * p.kv_heads * ((p.group + HEADS - 1) / HEADS) * p.splits;
   if (grid > 0x7FFFFFFFLL) return fail(MUSC_B200_ERR_INVALID, "masked_attention: too many rows and heads");
-  if (p.splits > 1 && p.splits <= MAX_CLUSTER) return launch_as<D, FP16, true>(p, grid, s);
-  return launch_as<D, FP16, false>(p, grid, s);
+  const bool cluster = p.splits > 1 && p.splits <= MAX_CLUSTER;
+  if (p.block_rows > 1)
+    return cluster ? launch_as<D, FP16, true, true>(p, grid, s) : launch_as<D, FP16, false, true>(p, grid, s);
+  return cluster ? launch_as<D, FP16, true, false>(p, grid, s) : launch_as<D, FP16, false, false>(p, grid, s);
 }
 
 }  // namespace
+
+int rows_together(int group, bool several) { return several ? std::max(1, HEADS / group) : 1; }
 
 int rows_splits(long long units, long long keys, bool single) {
   const long long target = single ? TARGET_SINGLE : TARGET_SEVERAL;

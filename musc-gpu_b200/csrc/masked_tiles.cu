@@ -149,11 +149,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&t);
 }
 
-template <bool FP16>
-__device__ __forceinline__ float widen(uint16_t v) {
-  return FP16 ? __half2float(__ushort_as_half(v)) : __bfloat162float(__ushort_as_bfloat16(v));
-}
-
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
@@ -198,7 +193,7 @@ __device__ __forceinline__ float here(float v) {
 
 // s -> cap2 * tanh(s / cap) for a row's tile (factor = scale / cap, cap2 = cap log2(e)).  The exact form
 // takes two of the special-function unit's operations an element, and the exponential a
-// third: 3072 cycles a half's tile where the unit bounds the kernel.  tanh(x) / x as a
+// third, where that unit already bounds the loop.  tanh(x) / x as a
 // polynomial in x^2 takes multiply-adds instead, two elements an instruction: of degree 3
 // where the warp's scores stay within |x| <= 0.4 (most do: a cap is chosen well above them),
 // of degree 6 up to 1, each fitted for the least maximum error (2e-8 and 2e-8 of tanh, below
@@ -283,22 +278,7 @@ __device__ __forceinline__ void rows_key_by_key(const Params& p, const int2* seg
     Walk walk(segments, first, last);
     int begin, end;
     while (walk.next(begin, end)) {
-      for (int key = max(begin, lo); key < min(end, hi); ++key) {
-        const uint16_t* k = static_cast<const uint16_t*>(p.k) + key * p.k_stride + kv_head * D + lane * N;
-        const uint16_t* v = static_cast<const uint16_t*>(p.v) + key * p.v_stride + kv_head * D + lane * N;
-        float dot = 0.f;
-        for (int i = 0; i < N; ++i) dot = fmaf(qf[i], widen<FP16>(k[i]), dot);
-        dot = warp_sum(dot);
-        float z = p.cap > 0.f ? capped_log2(dot, p.scale / p.cap, p.cap * LOG2E) : dot * p.scale * LOG2E;
-        if (p.slopes) z = fmaf(-slope2, fabsf((float)(key - pos)), z);
-        const float m_new = fmaxf(m, z);
-        const float a = m == -INFINITY ? 0.f : ex2(m - m_new);
-        m = m_new;
-        // a key whose score is -inf or has no weight left adds nothing, NaN scores add NaN
-        const float e = z == -INFINITY ? 0.f : ex2(z - m);
-        l = fmaf(l, a, e);
-        for (int i = 0; i < N; ++i) acc[i] = fmaf(e, widen<FP16>(v[i]), acc[i] * a);
-      }
+      attend_keys<D, FP16>(p, qf, kv_head, slope2, pos, max(begin, lo), min(end, hi), acc, m, l);
     }
     const long long at = (split * p.q_rows + row) * p.heads + head;
     if (p.splits == 1) {

@@ -361,6 +361,51 @@ def test_attention_split_documents(cuda_device, n_q, poison, d):
         _assert_close(got[n_q - 2:n_q][:, others], want[n_q - 2:n_q][:, others], tol[n_q - 2:n_q][:, others])
 
 
+@pytest.mark.parametrize('heads,kv_heads,d', [(1, 1, 64), (6, 2, 128), (5, 1, 64), (9, 1, 64), (16, 1, 128), (17, 1, 64)])
+@pytest.mark.parametrize('keys', [3, 700, 9000])
+@pytest.mark.parametrize('options', [{}, dict(causal=True), dict(causal=True, bias=True, softcap=8.0, prefix=True)])
+def test_attention_few_rows_of_each_document(cuda_device, heads, kv_heads, d, keys, options):
+    from musc_b200 import ops
+    docs = [(n, keys + n % 5) for n in (2, 1, 15, 0, 3, 16, 7, 4, 9, 31, 5)]
+    options, dtype = dict(options), torch.bfloat16 if heads % 2 else torch.float16
+    q_off, k_off = _starts([n for n, _ in docs]), _starts([m for _, m in docs])
+    q, k, v = _random_qkv(cuda_device, q_off[-1], k_off[-1], heads, kv_heads, d, dtype, 7 * keys + heads, False)
+    prefix = [m - n // 2 for n, m in docs] if options.pop('prefix', False) else None
+    slopes = 2.0 ** (-torch.arange(1, heads + 1, device=cuda_device).float()) if options.pop('bias', False) else None
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               prefix=None if prefix is None else _i32(prefix, cuda_device), slopes=slopes, **options)
+    _assert_close(got, *_reference(q, k, v, heads, kv_heads, q_off, k_off, prefix=prefix, slopes=slopes, **options))
+
+
+@pytest.mark.parametrize('poison', [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize('keys', [40, 5000])
+@pytest.mark.parametrize('bias', [False, True])
+def test_attention_last_keys_reach_only_the_rows_behind_them(cuda_device, keys, poison, bias):
+    """Rows of one document that share a product: values that are not finite at the last keys stay with the
+    rows that see them."""
+    from musc_b200 import ops
+    n, heads, d = 6, 4, 128
+    q, k, v = _random_qkv(cuda_device, n, keys, heads, 2, d, torch.float16, keys, False)
+    v = v.clone()
+    v[keys - 2, ::3] = poison  # seen by the last two rows
+    slopes = torch.tensor([0.5, 0.25, 0.0, 1.0], device=cuda_device) if bias else None
+    got = ops.attention_masked(q, k, v, heads, 2, offsets=_i32([0, n], cuda_device), kv_offsets=_i32([0, keys], cuda_device),
+                               causal=True, slopes=slopes)
+    clean = v.clone()
+    clean[keys - 2] = 0
+    want, tol = _reference(q, k, clean, heads, 2, [0, n], [0, keys], causal=True, slopes=slopes)
+    _assert_close(got[:n - 2], want[:n - 2], tol[:n - 2])
+    hit = torch.arange(d * 2, device=cuda_device) % 3 == 0
+    hit = torch.cat([hit[:d], hit[:d], hit[d:], hit[d:]])  # two heads for each key head
+    assert not bool(got[n - 2:, hit].isfinite().any())
+    assert bool(got[n - 2:, ~hit].isfinite().all())
+    k = k.clone()
+    k[keys - 1] = poison  # its scores reach the last row alone
+    got = ops.attention_masked(q, k, clean, heads, 2, offsets=_i32([0, n], cuda_device), kv_offsets=_i32([0, keys], cuda_device),
+                               causal=True, slopes=slopes)
+    _assert_close(got[:n - 1], want[:n - 1], tol[:n - 1])
+
+
 @pytest.mark.parametrize('n', [20, 900])
 def test_attention_disordered_offsets_stay_inside(cuda_device, n):
     """Offsets that fall, repeat or leave the tensors: results are undefined, accesses are not."""
