@@ -96,7 +96,7 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
     plan.block_rows = rows_together(group, a.q_rows > a.documents);
     const long long used = std::min<long long>(plan.block_rows, (a.q_rows + a.documents - 1) / a.documents);
     plan.splits = rows_splits((a.q_rows + used - 1) / used * a.kv_heads * ((group + 15) / 16), mean_keys(a),
-                              a.q_rows <= a.documents * used);
+                              (int)used * std::min(group, 16), a.head_dim);
   }
   if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {
     plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;

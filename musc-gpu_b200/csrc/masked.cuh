@@ -186,7 +186,7 @@ __device__ __forceinline__ float inverse_sum(float l, bool any_key) {
 constexpr int MAX_CLUSTER = 8;  // up to so many splits the row kernel joins by itself, without a workspace
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int rows_together(int group, bool several);  // several: rows a document
-int rows_splits(long long units, long long keys, bool single);  // single: documents of one block of rows each
+int rows_splits(long long units, long long keys, int rows, int head_dim);  // rows: of a block's products
 int tiles_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int tiles_splits(long long units, long long keys, bool causal);
 bool tiles_aligned(const Params& p);

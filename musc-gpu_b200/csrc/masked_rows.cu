@@ -25,13 +25,12 @@ constexpr int THREADS = WARPS * 32;
 constexpr int KEYS = 16;    // keys of a warp's step
 constexpr int STAGES = 2;   // steps in flight per warp: WARPS x STAGES x 64 D bytes a CTA
 constexpr int HEADS = 16;   // rows of the products: rows x query heads of a CTA
-// Splits.  Three waves of what is resident (148 SMs x 3 CTAs) even out documents of differing lengths:
-// 32 tokens over 8192 keys in 116 us, 132 with one wave.  Where several rows of a document read its keys
-// from L2, one wave keeps them together: 2 rows over 6390 keys in 32 us, 38 with three.
-constexpr int TARGET_SINGLE = 1332, TARGET_SEVERAL = 444;
-constexpr int MIN_KEYS = 256;       // of a split: 465 keys in one take 15 us, in two 21
-constexpr int CLUSTER_KEYS = 4096;  // more keys per split than this, and more than a cluster's splits are taken
+constexpr int MAX_SPLITS = 64;  // combine_kernel's two a lane
 constexpr float RESCALE = 8.f;  // log2 by which a running maximum may lag behind before sums are rescaled
+
+// CTAs of an SM: 73 KB of shared memory at D = 128, 128 registers a thread at D = 64.
+template <int D>
+constexpr int RESIDENT = D == 64 ? 4 : 3;
 
 template <int D>
 struct Smem {
@@ -135,8 +134,10 @@ __device__ __forceinline__ int find_block(const Params& p, long long block, long
   return row >= 0 && row < min((long long)__ldg(p.q_offsets + doc + 1), p.q_rows) ? doc : -1;
 }
 
+// Clusters keep the compiler's own choice of registers, at most as many: 32 tokens over 8192 keys in 120 us, 122
+// with the bound that the form without them needs (170 registers at D = 128, two CTAs an SM).
 template <int D, bool FP16, bool CLUSTER, bool SEVERAL>
-__global__ void __launch_bounds__(THREADS, D == 64 ? 4 : 3) rows_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, CLUSTER ? 0 : RESIDENT<D>) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem<D>& sm = *reinterpret_cast<Smem<D>*>(smem_raw);
   constexpr int CHUNKS = D / 8;  // 16-byte chunks of a key
@@ -433,11 +434,27 @@ int launch(const Params& p, cudaStream_t s) {
 
 int rows_together(int group, bool several) { return several ? std::max(1, HEADS / group) : 1; }
 
-int rows_splits(long long units, long long keys, bool single) {
-  const long long target = single ? TARGET_SINGLE : TARGET_SEVERAL;
-  const long long want = (target + units - 1) / units;
-  const long long splits = std::max<long long>(1, std::min<long long>(std::min<long long>(want, keys / MIN_KEYS), 64));
-  return (int)(splits > MAX_CLUSTER && keys <= MAX_CLUSTER * CLUSTER_KEYS ? MAX_CLUSTER : splits);
+// Splits of the keys of `units` blocks of rows: those whose time is least, by a model in keys' times
+// (9 ns at D = 128) fitted to 18 shapes in 1 to 8 splits, of which it takes one within 7 % of the best.
+// A CTA takes its keys, 128 to start and 20 a row for the join, once for each wave of them; a split 20
+// more, the grid 100 for each fill of the GPU, and more splits than a cluster's eight a second launch
+// that reads them all.
+//   2 rows over 6390 keys of 7 requests, 56 units: 392 CTAs 25.1 us, 448 (444 are resident) 32.5
+//   553 keys of 12 requests, 24 units: in one split 10.6 us, in two 8.7, in five 6.8
+//   15 rows x heads over 450 keys, 56 units: 10.6 us in one, 11.5 in two, 18.2 in seven
+//   8 rows over 20000 keys of 2 requests, 8 units: 39 us in eight, 27 in sixteen
+//   one row over 60000 keys, 8 units: 52 us in sixteen, 49 in 32, 56 in 52
+int rows_splits(long long units, long long keys, int rows, int head_dim) {
+  const long long resident = 148LL * (head_dim == 64 ? RESIDENT<64> : RESIDENT<128>);
+  int best = 1;
+  long long least = 0;
+  for (int splits = 1; splits <= MAX_SPLITS; ++splits) {
+    const long long ctas = units * splits, waves = (ctas + resident - 1) / resident;
+    const long long time = waves * (128 + (keys + splits - 1) / splits + (splits > 1 ? 20 * rows : 0)) + 100 * ctas / resident +
+                           (splits > MAX_CLUSTER ? 450 + 40 * splits : 20 * splits);
+    if (splits == 1 || time < least) least = time, best = splits;
+  }
+  return best;
 }
 
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t s) {
