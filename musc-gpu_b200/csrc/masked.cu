@@ -3,6 +3,7 @@
 #include "masked.cuh"
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 namespace musc {
@@ -83,21 +84,36 @@ long long mean_keys(const musc_b200_masked_attention_args& a) {
   return a.q_offsets ? (a.kv_rows + a.documents - 1) / a.documents : a.kv_len;
 }
 
+// Whether the tile kernel is the faster one, by estimates in microseconds of mean documents that were fitted to
+// 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys): 0.6 % over the faster of both in the mean, at
+// most 1.39 times.  A CTA of the row kernel takes up to 16 rows x heads of one document and key head, all resident
+// CTAs read keys together, and a lone document's keys still cost a part of that; one of the tile kernel takes 256
+// rows of one head over the keys of all documents in them, and starts slowly.
+//   61 rows of 8 documents, 4 heads x 128: rows 6.7 us, tiles 16.4
+//   1020 rows of 129 documents, 1 head x 64: rows 267 us, tiles 100
+//   12 rows of 403 documents, 16 heads x 128: rows 113 us, tiles 57
+bool tiles_faster(const musc_b200_masked_attention_args& a, long long units) {
+  const double keys = (double)mean_keys(a), rows = std::max(1.0, (double)a.q_rows / a.documents);
+  const double fill = units / (a.head_dim == 64 ? 592.0 : 444.0);
+  const double rows_time = 2 + 3 * std::max(1.0, fill) + (fill + 0.12) * keys * (a.head_dim == 64 ? 0.0075 : 0.0106);
+  const double tiles = rows < 256 ? std::ceil(a.q_rows / 256.0) : a.documents * std::ceil(rows / 256);
+  const double tile_keys = rows < 256 ? keys * std::min((double)a.documents, std::ceil(256 / rows)) : keys;
+  return 10 + (2 + 0.7 * tile_keys / 64) * tiles * a.heads / 148 < rows_time;
+}
+
 Plan make_plan(const musc_b200_masked_attention_args& a) {
   Plan plan;
   const long long rows = a.q_rows * a.heads;
   const int group = a.heads / a.kv_heads;
-  // A CTA of the tile kernel takes 256 rows of one head, one of the row kernel up to 16 rows x heads of
-  // one document and key head.
-  plan.tiles = a.kv_rows > 0 && a.q_rows >= 16LL * a.documents;
+  plan.block_rows = rows_together(group, a.q_rows > a.documents);
+  const long long mean_rows = (a.q_rows + a.documents - 1) / a.documents;
+  const long long used = std::min<long long>(plan.block_rows, mean_rows);
+  const long long units = a.documents * ((mean_rows + used - 1) / used) * a.kv_heads * ((group + 15) / 16);
+  plan.tiles = a.kv_rows > 0 && tiles_faster(a, units);
   if (plan.tiles)
     plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a), a.causal != 0);
-  else {
-    plan.block_rows = rows_together(group, a.q_rows > a.documents);
-    const long long used = std::min<long long>(plan.block_rows, (a.q_rows + a.documents - 1) / a.documents);
-    plan.splits = rows_splits((a.q_rows + used - 1) / used * a.kv_heads * ((group + 15) / 16), mean_keys(a),
-                              (int)used * std::min(group, 16), a.head_dim);
-  }
+  else
+    plan.splits = rows_splits(units, mean_keys(a), (int)used * std::min(group, 16), a.head_dim);
   if (plan.splits > (plan.tiles ? 1 : MAX_CLUSTER)) {
     plan.ml_offset = ((size_t)plan.splits * rows * a.head_dim * sizeof(float) + 255) / 256 * 256;
     plan.bytes = plan.ml_offset + (size_t)plan.splits * rows * sizeof(float2);

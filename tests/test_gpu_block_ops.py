@@ -406,6 +406,83 @@ def test_attention_last_keys_reach_only_the_rows_behind_them(cuda_device, keys, 
     _assert_close(got[:n - 1], want[:n - 1], tol[:n - 1])
 
 
+def _of_heads(t, d, first, count):
+    return t[:, first * d:(first + count) * d]
+
+
+@pytest.mark.parametrize('case', [i for i, c in enumerate(CASES) if sum(n for n, _ in c[0]) >= 16])
+def test_attention_of_many_heads(cuda_device, case):
+    """The same documents with 128 and more key heads, of which the first and the last are compared."""
+    from musc_b200 import ops
+    docs, heads, kv_heads, d, options = CASES[case]
+    options, dtype, group = dict(options), torch.bfloat16 if case % 2 else torch.float16, heads // kv_heads
+    kv_heads, heads = 128, 128 * group
+    q_off, k_off = _starts([n for n, _ in docs]), _starts([m for _, m in docs])
+    q, k, v = _random_qkv(cuda_device, q_off[-1], k_off[-1], heads, kv_heads, d, dtype, 900 + case, False)
+    slopes = 2.0 ** (-(torch.arange(heads, device=cuda_device) % 9).float()) if options.pop('bias', False) else None
+    prefix = options.pop('prefix', None)
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               prefix=None if prefix is None else _i32(prefix, cuda_device), slopes=slopes, **options)
+    for h in (0, kv_heads - 1):
+        part = None if slopes is None else slopes[h * group:(h + 1) * group]
+        want, tol = _reference(_of_heads(q, d, h * group, group), _of_heads(k, d, h, 1), _of_heads(v, d, h, 1), group, 1,
+                               q_off, k_off, prefix=prefix, slopes=part, **options)
+        _assert_close(_of_heads(got, d, h * group, group), want, tol)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('poison', [math.nan, math.inf, -math.inf])
+def test_attention_of_many_heads_masked_values_do_not_leak(cuda_device, poison, d):
+    """Documents of 300, 40 and 170 rows; the second one's last key and what lies behind the third's are not finite."""
+    from musc_b200 import ops
+    heads, lengths = 160, [300, 40, 170]
+    off = _starts(lengths)
+    q, k, v = _random_qkv(cuda_device, off[-1] + 30, off[-1] + 30, heads, heads, d, torch.float16, d, False)
+    k, v = k.clone(), v.clone()
+    k[off[2] - 1], v[off[2] - 1], k[off[3]:], v[off[3]:] = poison, poison, poison, poison
+    got = ops.attention_masked(q, k, v, heads, heads, offsets=_i32(off, cuda_device), causal=True)
+    clean_k, clean_v = k.clone(), v.clone()
+    clean_k[off[2] - 1], clean_v[off[2] - 1] = 0, 0
+    rows = torch.arange(off[-1], device=cuda_device) != off[2] - 1
+    for h in (0, heads // 2, heads - 1):
+        want, tol = _reference(*(_of_heads(t, d, h, 1) for t in (q, clean_k, clean_v)), 1, 1, off, off, causal=True)
+        _assert_close(_of_heads(got, d, h, 1)[:off[-1]][rows], want[:off[-1]][rows], tol[:off[-1]][rows])
+    assert not bool(got[off[2] - 1].isfinite().any())
+
+
+@pytest.mark.parametrize('n,rows,heads,kv_heads,d', [(400, 12, 16, 16, 128), (290, 8, 16, 16, 64), (330, 3, 32, 16, 128),
+                                                     (1500, 5, 12, 4, 64)])
+def test_attention_many_short_documents_of_many_heads(cuda_device, n, rows, heads, kv_heads, d):
+    from musc_b200 import ops
+    lengths = [rows + (i % 3) - 1 for i in range(n)]
+    off = _starts(lengths)
+    q, k, v = _random_qkv(cuda_device, off[-1], off[-1], heads, kv_heads, d, torch.bfloat16, n, True)
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(off, cuda_device), causal=True)
+    group, last = heads // kv_heads, kv_heads - 1
+    want, tol = _reference(_of_heads(q, d, last * group, group), _of_heads(k, d, last, 1), _of_heads(v, d, last, 1), group, 1,
+                           off, off, causal=True)
+    _assert_close(_of_heads(got, d, last * group, group), want, tol)
+
+
+@pytest.mark.parametrize('n_q,n_k', [(40, 3000), (300, 700)])
+@pytest.mark.parametrize('causal', [False, True])
+def test_attention_cache_slots_of_many_heads(cuda_device, n_q, n_k, causal):
+    """Slots in use to differing lengths; NaN behind them."""
+    from musc_b200 import ops
+    b, heads, kv_heads, d = 3, 192, 96, 64
+    g = torch.Generator(device=cuda_device).manual_seed(n_q)
+    q = torch.randn(b, n_q, heads * d, generator=g, device=cuda_device).half()
+    k, v = (torch.randn(b, n_k, kv_heads * d, generator=g, device=cuda_device).half() for _ in range(2))
+    used = [n_k, n_k // 2 + 1, n_q - 7]
+    for i, n in enumerate(used):
+        k[i, n:], v[i, n:] = math.nan, math.nan
+    got = ops.attention_masked(q, k, v, heads, kv_heads, kv_lengths=_i32(used, cuda_device), causal=causal)
+    for i, n in enumerate(used):
+        h = kv_heads - 1
+        want, tol = _reference(q[i, :, h * 2 * d:], k[i, :n, h * d:], v[i, :n, h * d:], 2, 1, [0, n_q], [0, n], causal=causal)
+        _assert_close(got[i, :, h * 2 * d:], want, tol)
+
+
 @pytest.mark.parametrize('n', [20, 900])
 def test_attention_disordered_offsets_stay_inside(cuda_device, n):
     """Offsets that fall, repeat or leave the tensors: results are undefined, accesses are not."""
