@@ -108,7 +108,8 @@ Plan make_plan(const musc_b200_masked_attention_args& a) {
   plan.block_rows = rows_together(group, a.q_rows > a.documents);
   const long long mean_rows = (a.q_rows + a.documents - 1) / a.documents;
   const long long used = std::min<long long>(plan.block_rows, mean_rows);
-  const long long units = a.documents * ((mean_rows + used - 1) / used) * a.kv_heads * ((group + 15) / 16);
+  // documents that have rows: at most as many as there are rows
+  const long long units = std::min<long long>(a.documents, a.q_rows) * ((mean_rows + used - 1) / used) * a.kv_heads * ((group + 15) / 16);
   plan.tiles = a.kv_rows > 0 && tiles_faster(a, units);
   if (plan.tiles)
     plan.splits = tiles_splits((a.q_rows + 255) / 256 * a.heads, mean_keys(a), a.causal != 0);

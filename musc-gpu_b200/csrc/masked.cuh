@@ -128,8 +128,8 @@ __device__ __forceinline__ float capped_log2(float s, float factor, float cap2) 
 }
 
 // log2 by which the stored exponentials are raised.  In fp16 a weight below 2^-24 of the row's
-// largest would be lost; raised by 2^6 (and up to 2^8 more while a running maximum lags, still
-// below 65504) it keeps 2^-30.  Sums carry the same factor, which cancels.  bf16 has fp32's range.
+// largest would be lost; raised by 2^6 (and by what a running maximum lags, which the kernels bound so
+// that sums of them stay below 65504) it keeps 2^-30.  Sums carry the same factor, which cancels.  bf16 has fp32's range.
 template <bool FP16>
 constexpr float RAISE = FP16 ? 6.f : 0.f;
 

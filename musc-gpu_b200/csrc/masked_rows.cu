@@ -1,14 +1,17 @@
 // Masked attention of few query rows against many keys (masked.cuh has the operator): one
-// CTA per query row (or a few of one document), key head and split of the keys.
+// CTA per block of rows of a document, key head and split of the keys.
 //
-// Keys and values are read once for all query heads of their group, and nothing else
-// is large: memory bounds it.  The group's heads, for as many consecutive rows of a document as fit, are
-// the 16 rows of the tensor core's m16n8k16 products (a larger group takes several CTAs): S = Q K^T over 16 keys and the head
-// dimension, then O += P V, at 2 x 16 x 16 x D operations per 64 D bytes far below what the
-// tensor cores give.  Each of the CTA's warps takes every WARPS-th run of 16 keys through a
+// Keys and values are read once for a block's rows and all query heads of their group, and nothing
+// else is large: memory bounds it.  The group's heads, for as many consecutive rows of a document as fit
+// (5 rows over 2985 keys of 20 requests in 16.8 us, 34 when each row read the keys for itself), are the
+// 16 rows of the tensor core's m16n8k16 products (a larger group takes several CTAs): S = Q K^T over 16
+// keys and the head dimension, then O += P V, at 2 x 16 x 16 x D operations per 64 D bytes far below
+// what the tensor cores give.  Each of the CTA's warps takes every WARPS-th run of 16 keys through a
 // ring of its own that cp.async fills STAGES runs ahead, so no barrier stands between a
-// warp's loads and their use; keys past the row's interval are filled with zeros by the copy
-// itself (a masked value that is NaN never reaches a product).  The warps' and the splits'
+// warp's loads and their use; keys past the rows' interval are filled with zeros by the copy
+// itself (a masked value that is NaN never reaches a product).  Under a causal mask the last keys
+// (fewer than 16) are seen by some of the block's rows only: they are a step of their own, and if a value
+// there is not finite the block's rows are taken again key by key.  The warps' and the splits'
 // sums are joined at the end by their maxima: up to eight splits form a cluster and read each
 // other's sums from shared memory (one launch, no workspace), more leave theirs to combine_kernel.
 #include "masked.cuh"
