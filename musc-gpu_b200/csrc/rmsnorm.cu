@@ -389,8 +389,9 @@ extern "C" int musc_b200_add_rmsnorm(void* x, int x_dtype, const void* delta, in
   };
   const Span sc = {reinterpret_cast<uintptr_t>(scales), rows * 4 * (group ? (channels + group - 1) / group : 1), 0, 4};
   const bool eight = out_dtype == MUSC_B200_E4M3;
+  if (eight && sc.at % 4 != 0) return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: scales must be aligned to 4 bytes");
   if (meet(so, sx) || meet(so, sw) || (delta && meet(sx, sw)) || (delta && (meet(so, sd) || meet(sx, sd))) ||
-      (eight && (meet(sc, sx) || meet(sc, so) || (delta && meet(sc, sd)))))
+      (eight && (meet(sc, sx) || meet(sc, so) || meet(sc, sw) || (delta && meet(sc, sd)))))
     return fail(MUSC_B200_ERR_INVALID, "add_rmsnorm: x, delta, weight, out and scales must not overlap");
   MUSC_TRY(require_sm100());
   Params p;

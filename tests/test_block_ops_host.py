@@ -120,6 +120,12 @@ def test_norm_contract(changes, message):
     assert _norm(**changes) == _lib.ERR_INVALID and message in _lib.last_error()
 
 
+@pytest.mark.parametrize('changes,message', [(dict(scales=(5 << 20) + 2), 'scales must be aligned'),
+                                             (dict(scales=(3 << 20) + 8), 'overlap')])
+def test_norm_scales_contract(changes, message):
+    assert _norm(**changes) == _lib.ERR_INVALID and message in _lib.last_error()
+
+
 def test_norm_without_rows():
     assert _norm(rows=0, x=None) == _lib.OK
 
