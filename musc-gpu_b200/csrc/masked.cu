@@ -86,16 +86,19 @@ long long mean_keys(const musc_b200_masked_attention_args& a) {
 
 // Whether the tile kernel is the faster one, by estimates in microseconds of mean documents that were fitted to
 // 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys): 0.6 % over the faster of both in the mean, at
-// most 1.39 times.  A CTA of the row kernel takes up to 16 rows x heads of one document and key head, all resident
+// most 1.39 times; on 110 others 1.0 % and 1.51 times.  A CTA of the row kernel takes up to 16 rows x heads of one document and key head, all resident
 // CTAs read keys together, and a lone document's keys still cost a part of that; one of the tile kernel takes 256
 // rows of one head over the keys of all documents in them, and starts slowly.
 //   61 rows of 8 documents, 4 heads x 128: rows 6.7 us, tiles 16.4
 //   1020 rows of 129 documents, 1 head x 64: rows 267 us, tiles 100
 //   12 rows of 403 documents, 16 heads x 128: rows 113 us, tiles 57
+//   8 rows over 20000 keys of 2 documents, 8 heads on one key head x 128: rows 26 us, tiles 42
 bool tiles_faster(const musc_b200_masked_attention_args& a, long long units) {
   const double keys = (double)mean_keys(a), rows = std::max(1.0, (double)a.q_rows / a.documents);
   const double fill = units / (a.head_dim == 64 ? 592.0 : 444.0);
-  const double rows_time = 2 + 3 * std::max(1.0, fill) + (fill + 0.12) * keys * (a.head_dim == 64 ? 0.0075 : 0.0106);
+  // a lone unit's keys in eight splits, or in as many as pay (40 keys' times each, and the second launch)
+  const double lone = std::min(0.12 * keys, 450 + 2 * std::sqrt(40 * keys));
+  const double rows_time = 2 + 3 * std::max(1.0, fill) + (fill * keys + lone) * (a.head_dim == 64 ? 0.0075 : 0.0106);
   const double tiles = rows < 256 ? std::ceil(a.q_rows / 256.0) : a.documents * std::ceil(rows / 256);
   const double tile_keys = rows < 256 ? keys * std::min((double)a.documents, std::ceil(256 / rows)) : keys;
   return 10 + (2 + 0.7 * tile_keys / 64) * tiles * a.heads / 148 < rows_time;
