@@ -84,11 +84,11 @@ long long mean_keys(const musc_b200_masked_attention_args& a) {
   return a.q_offsets ? (a.kv_rows + a.documents - 1) / a.documents : a.kv_len;
 }
 
-// Whether the tile kernel is the faster one, by estimates in microseconds of mean documents that were fitted to
-// 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys): 0.6 % over the faster of both in the mean, at
-// most 1.39 times; on 110 others 1.0 % and 1.51 times.  A CTA of the row kernel takes up to 16 rows x heads of one document and key head, all resident
-// CTAs read keys together, and a lone document's keys still cost a part of that; one of the tile kernel takes 256
-// rows of one head over the keys of all documents in them, and starts slowly.
+// Whether the tile kernel is the faster one, by estimates in microseconds for mean documents that were
+// fitted to 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys): 0.6 % over the faster of
+// both in the mean, at most 1.39 times; on 110 others 1.0 % and 1.51 times.  A CTA of the row kernel takes up
+// to 16 rows x heads of one document and key head; one of the tile kernel takes 256 rows of one head over the
+// keys of all documents in them, and starts slowly.
 //   61 rows of 8 documents, 4 heads x 128: rows 6.7 us, tiles 16.4
 //   1020 rows of 129 documents, 1 head x 64: rows 267 us, tiles 100
 //   12 rows of 403 documents, 16 heads x 128: rows 113 us, tiles 57

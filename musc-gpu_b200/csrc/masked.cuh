@@ -140,19 +140,20 @@ __device__ __forceinline__ float widen(uint16_t v) {
 
 // A row and head's sums over keys [first, end) by a warp, key by key: lanes hold D / 32 dimensions of q and
 // of the sums.  The slow form, for rows beside values that are not finite and that they do not see.
-template <int D, bool FP16>
-__device__ __forceinline__ void attend_keys(const Params& p, const float (&q)[D / 32], int kv_head, float slope2, long long pos,
-                                            long long first, long long end, float (&acc)[D / 32], float& m, float& l) {
+// Index: of keys and their distances.
+template <int D, bool FP16, typename Index>
+__device__ __forceinline__ void attend_keys(const Params& p, const float (&q)[D / 32], int kv_head, float slope2, Index pos,
+                                            int first, int end, float (&acc)[D / 32], float& m, float& l) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
-  for (long long key = first; key < end; ++key) {
+  for (int key = first; key < end; ++key) {
     const uint16_t* k = static_cast<const uint16_t*>(p.k) + key * p.k_stride + kv_head * D + lane * N;
     const uint16_t* v = static_cast<const uint16_t*>(p.v) + key * p.v_stride + kv_head * D + lane * N;
     float dot = 0.f;
     for (int i = 0; i < N; ++i) dot = fmaf(q[i], widen<FP16>(k[i]), dot);
     dot = warp_sum(dot);
     float z = p.cap > 0.f ? capped_log2(dot, p.scale / p.cap, p.cap * LOG2E) : dot * p.scale * LOG2E;
-    if (p.slopes) z = fmaf(-slope2, (float)llabs(key - pos), z);
+    if (p.slopes) z = fmaf(-slope2, fabsf((float)(key - pos)), z);
     const float m_new = fmaxf(m, z);
     const float a = m == -INFINITY ? 0.f : ex2(m - m_new);
     m = m_new;

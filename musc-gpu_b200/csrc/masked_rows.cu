@@ -137,8 +137,8 @@ __device__ __forceinline__ int find_block(const Params& p, long long block, long
   return row >= 0 && row < min((long long)__ldg(p.q_offsets + doc + 1), p.q_rows) ? doc : -1;
 }
 
-// Clusters keep the compiler's own choice of registers, at most as many: 32 tokens over 8192 keys in 120 us, 122
-// with the bound that the form without them needs (170 registers at D = 128, two CTAs an SM).
+// The form with clusters keeps the compiler's own choice of registers (168 at D = 128): with the bound that the form
+// without them needs (170 registers else, two CTAs an SM), 32 tokens over 8192 keys take 1.5 % longer.
 template <int D, bool FP16, bool CLUSTER, bool SEVERAL>
 __global__ void __launch_bounds__(THREADS, CLUSTER ? 0 : RESIDENT<D>) rows_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(THREADS, CLUSTER ? 0 : RESIDENT<D>) rows_kerne
       for (int i = 0; i < N; ++i) qf[i] = widen<FP16>(q[i]), acc[i] = 0.f;
       const float slope = p.slopes ? __ldg(p.slopes + h) * LOG2E : 0.f;
       const int main_last = min(last, main_steps);
-      const long long own = interval_end(p, iv, t);
+      const int own = (int)interval_end(p, iv, t);
       if (first < main_last)
         attend_keys<D, FP16>(p, qf, kv_head, slope, iv.pos + t, step_key(first), min(step_key(main_last - 1) + KEYS, common), acc,
                              m_row, l_row);
@@ -440,7 +440,7 @@ int rows_together(int group, bool several) { return several ? std::max(1, HEADS 
 // Splits of the keys of `units` blocks of rows: those whose time is least, by a model in keys' times
 // (9 ns at D = 128) fitted to 18 shapes in 1 to 8 splits, of which it takes one within 7 % of the best.
 // A CTA takes its keys, 128 to start and 20 a row for the join, once for each wave of them; a split 20
-// more, the grid 100 for each fill of the GPU, and more splits than a cluster's eight a second launch
+// more, the grid 130 for each fill of the GPU, and more splits than a cluster's eight a second launch
 // that reads them all.
 //   2 rows over 6390 keys of 7 requests, 56 units: 392 CTAs 25.1 us, 448 (444 are resident) 32.5
 //   553 keys of 12 requests, 24 units: in one split 10.6 us, in two 8.7, in five 6.8
@@ -453,7 +453,7 @@ int rows_splits(long long units, long long keys, int rows, int head_dim) {
   long long least = 0;
   for (int splits = 1; splits <= MAX_SPLITS; ++splits) {
     const long long ctas = units * splits, waves = (ctas + resident - 1) / resident;
-    const long long time = waves * (128 + (keys + splits - 1) / splits + (splits > 1 ? 20 * rows : 0)) + 100 * ctas / resident +
+    const long long time = waves * (128 + (keys + splits - 1) / splits + (splits > 1 ? 20 * rows : 0)) + 130 * ctas / resident +
                            (splits > MAX_CLUSTER ? 450 + 40 * splits : 20 * splits);
     if (splits == 1 || time < least) least = time, best = splits;
   }
