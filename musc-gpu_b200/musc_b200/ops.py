@@ -541,6 +541,11 @@ def _at(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _packed_like(t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """A contiguous tensor of ``t``'s shape (3 us less than ``torch.empty`` of its shape, type and device)."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _token_rows(what: str, name: str, t: torch.Tensor) -> tuple[int, int, int]:
     """``(rows, row stride, rows between batch items)`` of a token-major ``(T, W)`` or ``(B, L, W)`` tensor."""
     shape, stride = t.shape, t.stride()
@@ -620,7 +625,7 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     if q.ndim == 3 and (q_pitch != q.shape[1] or v_pitch != kv_pitch):
         raise ValueError('attention_masked: batch items of q must follow each other, those of k and v lie equally far apart')
     if out is None:
-        out, out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), heads * head_dim
+        out, out_stride = _packed_like(q), heads * head_dim
     else:
         if out.shape != q.shape or out.dtype != q.dtype:
             raise ValueError('attention_masked: out must have the shape and type of q')
@@ -708,9 +713,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     q_stride, k_stride = row_stride('q', q), 0 if k is None else row_stride('k', k)
     k_out, k_out_stride = None, kv_heads * head_dim
     if out is None:
-        q_out, q_out_stride = torch.empty(q.shape, dtype=q.dtype, device=dev), width
+        q_out, q_out_stride = _packed_like(q), width
         if k is not None:
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=dev)
+            k_out = _packed_like(k)
     else:
         _on_device(what, dev, q_out=out[0], k_out=out[1])
         for t, o in ((q, out[0]), (k, out[1])):
@@ -763,7 +768,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
     if group not in (0, 32, 64, 128, 256) or (group and not eight):
         raise ValueError('add_rmsnorm: group must be 0, or 32, 64, 128 or 256 for a float8_e4m3fn output')
     if out is None:
-        out = torch.empty(x.shape, dtype=out_dtype, device=dev)
+        out = _packed_like(x, out_dtype)
     if out.shape != x.shape or out.dtype != out_dtype:
         raise ValueError('add_rmsnorm: out must have the shape of x and type out_dtype')
     if eight:
