@@ -450,11 +450,11 @@ int rows_together(int group, bool several) { return several ? std::max(1, HEADS 
 int rows_splits(long long units, long long keys, int rows, int head_dim) {
   const long long resident = 148LL * (head_dim == 64 ? RESIDENT<64> : RESIDENT<128>);
   int best = 1;
-  long long least = 0;
+  double least = 0;
   for (int splits = 1; splits <= MAX_SPLITS; ++splits) {
     const long long ctas = units * splits, waves = (ctas + resident - 1) / resident;
-    const long long time = waves * (128 + (keys + splits - 1) / splits + (splits > 1 ? 20 * rows : 0)) + 130 * ctas / resident +
-                           (splits > MAX_CLUSTER ? 450 + 40 * splits : 20 * splits);
+    const double time = (double)waves * (128 + (keys + splits - 1) / splits + (splits > 1 ? 20 * rows : 0)) +
+                        130 * ctas / resident + (splits > MAX_CLUSTER ? 450 + 40 * splits : 20 * splits);
     if (splits == 1 || time < least) least = time, best = splits;
   }
   return best;
