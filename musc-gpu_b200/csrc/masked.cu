@@ -143,7 +143,8 @@ int check_args(const musc_b200_masked_attention_args& a) {
     if (!a.kv_offsets) return invalid("q_offsets and kv_offsets go together");
   } else {
     if (a.kv_offsets) return invalid("q_offsets and kv_offsets go together");
-    if (a.q_len < 0 || a.kv_len < 0 || a.kv_pitch < a.kv_len || a.q_len > a.q_rows || a.kv_pitch > 0x7FFFFFFF)
+    // (an empty batch has no rows, whatever its items' length)
+    if (a.q_len < 0 || a.kv_len < 0 || a.kv_pitch < a.kv_len || (a.documents > 0 && a.q_len > a.q_rows) || a.kv_pitch > 0x7FFFFFFF)
       return invalid("0 <= q_len <= q_rows and 0 <= kv_len <= kv_pitch < 2^31");
     if (a.q_len * a.documents != a.q_rows) return invalid("documents of q_len rows must make q_rows");
     if (a.documents > 0 && (a.documents - 1) * a.kv_pitch + a.kv_len > a.kv_rows)

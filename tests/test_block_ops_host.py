@@ -151,3 +151,15 @@ def test_rotary_frequencies():
     for bad in ([], [0, 0], [-1, 3]):
         with pytest.raises(ValueError):
             ops.rotary_frequencies(bad, device='cpu')
+
+
+@pytest.mark.parametrize('q_len,kv_len', [(70, 70), (1, 8192), (0, 0), (1 << 40, 5)])
+def test_attention_of_an_empty_batch(q_len, kv_len):
+    """A batch of no items has no rows, whatever the items' length."""
+    args = _attention_args(q=None, k=None, v=None, out=None, q_offsets=None, kv_offsets=None, documents=0, q_rows=0, kv_rows=0,
+                           q_len=q_len, kv_len=kv_len, kv_pitch=kv_len)
+    assert _lib.lib().musc_b200_masked_attention(ctypes.byref(args), None) == _lib.OK
+    assert _lib.lib().musc_b200_masked_attention_bytes(ctypes.byref(args)) == 0
+    args.documents = 1  # an item without its rows
+    if q_len:
+        assert _lib.lib().musc_b200_masked_attention(ctypes.byref(args), None) == _lib.ERR_INVALID
