@@ -464,6 +464,11 @@ typedef struct musc_b200_masked_attention_args {
  * q_offsets being NULL or not); 0 also for arguments that the call refuses. */
 size_t musc_b200_masked_attention_bytes(const musc_b200_masked_attention_args* args);
 
+/* What a call with these sizes runs, for tests and profiles (pointers as above): *tile_kernel
+ * 1 for the kernel of many query rows, 0 for the one of few; *splits the parts that each
+ * unit's keys are divided into (0: nothing runs). */
+int musc_b200_masked_attention_plan(const musc_b200_masked_attention_args* args, int* tile_kernel, int* splits);
+
 int musc_b200_masked_attention(const musc_b200_masked_attention_args* args, musc_b200_stream stream);
 
 /* ------------------------------------------------------------------------

@@ -190,6 +190,17 @@ extern "C" size_t musc_b200_masked_attention_bytes(const musc_b200_masked_attent
   return masked::make_plan(*args).bytes;
 }
 
+extern "C" int musc_b200_masked_attention_plan(const musc_b200_masked_attention_args* args, int* tile_kernel, int* splits) {
+  using namespace masked;
+  if (!args || !tile_kernel || !splits) return invalid("null arguments");
+  *tile_kernel = *splits = 0;
+  MUSC_TRY(check_args(*args));
+  if (args->q_rows == 0 || args->documents == 0) return MUSC_B200_OK;
+  const Plan plan = make_plan(*args);
+  *tile_kernel = plan.tiles, *splits = plan.splits;
+  return MUSC_B200_OK;
+}
+
 extern "C" int musc_b200_masked_attention(const musc_b200_masked_attention_args* args, musc_b200_stream stream) {
   using namespace masked;
   if (!args) return invalid("null arguments");

@@ -72,6 +72,7 @@ SIGNATURES = {
     'musc_b200_rotary': (_int, [_vp, _vp, _vp, _vp, _int, _ll, _int, _int, _int, _ll, _ll, _ll, _ll, _vp, _int, _int, _vp,
                                 _vp, _int, _int, _vp]),
     'musc_b200_masked_attention_bytes': (_sz, [ctypes.POINTER(MaskedAttentionArgs)]),
+    'musc_b200_masked_attention_plan': (_int, [ctypes.POINTER(MaskedAttentionArgs), ctypes.POINTER(_int), ctypes.POINTER(_int)]),
     'musc_b200_masked_attention': (_int, [ctypes.POINTER(MaskedAttentionArgs), _vp]),
     'musc_b200_preprocess_workspace_bytes': (_sz, [_int, _int, _int, _int, _int]),
     'musc_b200_preprocess_images': (_int, [_vp, _int, _int, _int, _ll, _int, _int, _int,

@@ -163,3 +163,32 @@ def test_attention_of_an_empty_batch(q_len, kv_len):
     args.documents = 1  # an item without its rows
     if q_len:
         assert _lib.lib().musc_b200_masked_attention(ctypes.byref(args), None) == _lib.ERR_INVALID
+
+
+def _plan(**changes):
+    """(tile kernel, splits) of a call."""
+    tiles, splits = ctypes.c_int(-1), ctypes.c_int(-1)
+    st = _lib.lib().musc_b200_masked_attention_plan(ctypes.byref(_attention_args(**changes)), ctypes.byref(tiles),
+                                                    ctypes.byref(splits))
+    assert st == _lib.OK, _lib.last_error()
+    return tiles.value, splits.value
+
+
+def test_attention_plan():
+    lib, one = _lib.lib(), ctypes.c_int(7)
+    assert lib.musc_b200_masked_attention_plan(None, ctypes.byref(one), ctypes.byref(one)) == _lib.ERR_INVALID
+    assert lib.musc_b200_masked_attention_plan(ctypes.byref(_attention_args()), None, ctypes.byref(one)) == _lib.ERR_INVALID
+    bad = _attention_args(head_dim=80)
+    assert lib.musc_b200_masked_attention_plan(ctypes.byref(bad), ctypes.byref(one), ctypes.byref(one)) == _lib.ERR_INVALID
+    assert _plan(q_rows=0) == (0, 0) and _plan(documents=0) == (0, 0)
+    assert _plan(kv_rows=0) == (0, 1)                                        # no keys: nothing to split
+    assert _plan(q_rows=8192, kv_rows=8192, heads=16, kv_heads=16, documents=1, causal=0) == (1, 1)
+    assert _plan(q_rows=32, kv_rows=32 * 8192, heads=32, kv_heads=8, documents=32)[0] == 0
+    # above eight splits the row kernel's sums go through the workspace, as the tile kernel's do above one
+    for sizes in (dict(q_rows=8, kv_rows=40_000, heads=8, kv_heads=1, head_dim=128, documents=2),
+                  dict(q_rows=512, kv_rows=8192, documents=1, causal=0)):
+        args = _attention_args(**sizes)
+        tiles, splits = _plan(**sizes)
+        assert splits > (1 if tiles else 8)
+        rows = sizes['q_rows'] * args.heads * splits
+        assert lib.musc_b200_masked_attention_bytes(ctypes.byref(args)) >= rows * (args.head_dim * 4 + 8)
