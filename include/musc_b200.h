@@ -433,8 +433,8 @@ int musc_b200_rotary(const void* q, const void* k, void* q_out, void* k_out, int
  * the key slot [kv_offsets[d], kv_offsets[d + 1]); or both NULL: documents of
  * q_len query rows each (documents * q_len == q_rows) with kv_len keys from row
  * d * kv_pitch on.  kv_lengths [documents] (nullable): keys in use at the start of
- * each slot.  Values outside the tensors are clamped to them.  Query rows
- * outside every document are not written.
+ * each slot.  Values outside the tensors are clamped to them (a document's rows too:
+ * its positions count the rows it has).  Query rows outside every document are not written.
  * scale from 1e-20 to 1e20, softcap 0 or from 1e-15 to 1e15.
  * out must not overlap q, k or v.  workspace: musc_b200_masked_attention_bytes
  * (0 if none is needed), 256-byte aligned, free for reuse once the stream has

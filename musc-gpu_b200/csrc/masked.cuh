@@ -63,6 +63,12 @@ __device__ __forceinline__ long long interval_end(const Params& p, const Interva
   return iv.lo + min(max(max(iv.pos + after + 1 - iv.lo, iv.least), 0LL), iv.keys);
 }
 
+// Packed rows before document d, cut to the rows there are: what an offset claims beyond them has no rows,
+// and none that would move a row's position.
+__device__ __forceinline__ int row_offset(const Params& p, int d) {
+  return (int)min(max((long long)__ldg(p.q_offsets + d), 0LL), p.q_rows);
+}
+
 // Document of a row: the last one that begins at or before it.  -1: the row belongs to none.
 __device__ __forceinline__ int find_document(const Params& p, long long row) {
   if (!p.q_offsets) return (int)(row / p.q_len);
@@ -79,8 +85,8 @@ __device__ __forceinline__ int find_document(const Params& p, long long row) {
 __device__ __forceinline__ Interval row_interval(const Params& p, int doc, long long row) {
   long long q0, nq, k0, nk;
   if (p.q_offsets) {
-    q0 = __ldg(p.q_offsets + doc);
-    nq = __ldg(p.q_offsets + doc + 1) - q0;
+    q0 = row_offset(p, doc);
+    nq = row_offset(p, doc + 1) - q0;
     k0 = min(max((long long)__ldg(p.kv_offsets + doc), 0LL), p.kv_rows);
     nk = min(max((long long)__ldg(p.kv_offsets + doc + 1), k0), p.kv_rows) - k0;
   } else {

@@ -113,7 +113,7 @@ __device__ __forceinline__ int find_block(const Params& p, long long block, long
     return doc;
   }
   const auto begin = [&](int d) {
-    const int first = __ldg(p.q_offsets + d);
+    const int first = row_offset(p, d);
     return SEVERAL ? (long long)(first / size) + d : (long long)first;
   };
   int doc;  // the last document that begins at or before the block
@@ -133,8 +133,8 @@ __device__ __forceinline__ int find_block(const Params& p, long long block, long
     doc = (int)__reduce_add_sync(0xffffffffu, before) - 1;
   }
   if (doc < 0) return -1;
-  row = SEVERAL ? __ldg(p.q_offsets + doc) + (block - begin(doc)) * size : block;
-  return row >= 0 && row < min((long long)__ldg(p.q_offsets + doc + 1), p.q_rows) ? doc : -1;
+  row = SEVERAL ? row_offset(p, doc) + (block - begin(doc)) * size : block;
+  return row >= 0 && row < row_offset(p, doc + 1) ? doc : -1;  // below 0: offsets out of order
 }
 
 // The form with clusters keeps the compiler's own choice of registers (168 at D = 128): with the bound that the form
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, CLUSTER ? 0 : RESIDENT<D>) rows_kerne
   const int doc = find_block<SEVERAL>(p, row_block, row);
   if (doc < 0) return;  // uniform over the CTA and its cluster
   const Interval iv = row_interval(p, doc, row);
-  const int n_tokens = SEVERAL ? (int)min(min((long long)p.block_rows, iv.rows_left), p.q_rows - row) : 1;
+  const int n_tokens = SEVERAL ? (int)min((long long)p.block_rows, iv.rows_left) : 1;
   const int n_rows = n_tokens * n_heads;  // row r: token r / n_heads, head r % n_heads
   // Keys that all of them see, in whole steps; then those that only the later ones do (fewer than a step).
   const int lo = (int)iv.lo, common = (int)iv.hi, end = (int)interval_end(p, iv, n_tokens - 1);

@@ -345,7 +345,7 @@ tiles_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ 
   // ------------------------------------------------ the CTA's rows, their intervals and its walk
   const bool shared_offsets = p.q_offsets && p.documents <= SHARED_DOCS;
   if (shared_offsets)
-    for (int i = threadIdx.x; i <= p.documents; i += THREADS) sm.offsets[i] = __ldg(p.q_offsets + i);
+    for (int i = threadIdx.x; i <= p.documents; i += THREADS) sm.offsets[i] = row_offset(p, i);
   if (threadIdx.x == 0) sm.tile_doc = -1;
   tc::fence_before_sync();
   __syncthreads();
