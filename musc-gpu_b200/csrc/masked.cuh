@@ -190,6 +190,7 @@ __device__ __forceinline__ float inverse_sum(float l, bool any_key) {
 
 // The kernels' launchers, and the splits of the keys that give `units` CTAs of work enough CTAs
 // when a document has about `keys` keys.
+constexpr int MAX_TILE_SPLITS = 32;
 constexpr int MAX_CLUSTER = 8;  // up to so many splits the row kernel joins by itself, without a workspace
 int rows_launch(const Params& p, int head_dim, bool fp16, cudaStream_t stream);
 int rows_together(int group, bool several);  // several: rows a document

@@ -878,7 +878,7 @@ int tiles_splits(long long units, long long keys, bool causal) {
   units = std::max<long long>(units, 1);
   long long splits = std::min<long long>(148 / units, keys / 256);
   if (causal) splits = std::max(splits, std::min<long long>((2 * 148 + units / 2) / units, keys / 2048));
-  return (int)std::max<long long>(1, std::min<long long>(splits, 32));
+  return (int)std::max<long long>(1, std::min<long long>(splits, MAX_TILE_SPLITS));
 }
 
 // Documents begin tiles of their own (long ones; runs of short ones share them) where they have 64 rows in

@@ -192,3 +192,15 @@ def test_attention_plan():
         assert splits > (1 if tiles else 8)
         rows = sizes['q_rows'] * args.heads * splits
         assert lib.musc_b200_masked_attention_bytes(ctypes.byref(args)) >= rows * (args.head_dim * 4 + 8)
+
+
+@pytest.mark.parametrize('head_dim', [64, 128])
+def test_attention_plan_of_long_contexts(head_dim):
+    """Few heads over very long keys: the tile kernel divides a row tile's keys into 32 at most, the row kernel into
+    64, so one row goes to the row kernel and 256 rows to the tile kernel, however long the keys."""
+    for keys in (300_000, 1_000_000):
+        for heads in (1, 2):
+            sizes = dict(kv_rows=keys, heads=heads, kv_heads=heads, head_dim=head_dim, documents=1)
+            tiles, splits = _plan(q_rows=1, **sizes)
+            assert tiles == 0 and splits > 32
+            assert _plan(q_rows=256, **dict(sizes, heads=2, kv_heads=1)) == (1, 32)
