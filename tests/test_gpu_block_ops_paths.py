@@ -62,3 +62,325 @@ def test_query_offsets_past_the_tensor(cuda_device, kernel, n, heads):
                                    causal=True, slopes=slopes)
         cut = [min(max(o, 0), n) for o in q_off]
         _assert_heads(got, q, k, v, heads, kv_heads, cut, k_off, causal=True, slopes=slopes)
+
+
+def test_empty_batches(cuda_device):
+    from musc_b200 import ops
+    x = torch.zeros(3, 70, 128, dtype=torch.float16, device=cuda_device)
+    assert ops.attention_masked(x[:0], x[:0], x[:0], 2, causal=True).shape == (0, 70, 128)
+    assert ops.attention_masked(x[:, :0], x, x, 2).shape == (3, 0, 128)
+    x[:] = 1
+    assert bool((ops.attention_masked(x, x[:, :0], x[:, :0], 2) == 0).all())
+
+
+# ----------------------------------------------------------------------------- the row kernel's sums in a workspace
+# rows and keys of the documents, heads, kv_heads, head_dim, splits (above, up to)
+LONG = [
+    ([(4, 30_000), (4, 30_000)], 8, 1, 128, (8, 32)),
+    ([(3, 20_011), (0, 5), (6, 40_000)], 2, 1, 64, (8, 32)),
+    ([(10, 100_000)], 4, 2, 64, (32, 64)),
+    ([(1, 100_000)], 1, 1, 64, (32, 64)),
+    ([(9, 200_003), (7, 197_001)], 6, 2, 128, (32, 64)),
+]
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('options', [{}, dict(causal=True, softcap=9.0, bias=True), dict(causal=True, prefix=True)])
+@pytest.mark.parametrize('case', range(len(LONG)))
+def test_rows_over_long_keys_in_many_splits(cuda_device, case, options, dtype):
+    """More splits than a cluster joins: unnormalised sums through the workspace.  Scores grow along the keys, so that
+    the splits' maxima differ; a document without keys gives zeros."""
+    from musc_b200 import ops
+    docs, heads, kv_heads, d, (above, most) = LONG[case]
+    options, empty = dict(options), (3, 0)
+    docs = docs + [empty]
+    q_off, k_off = _starts([n for n, _ in docs]), _starts([m for _, m in docs])
+    q, k, v = _random_qkv(cuda_device, q_off[-1], k_off[-1], heads, kv_heads, d, dtype, 200 + case, False)
+    k = (k.float() * torch.linspace(0.2, 2.0, k_off[-1], device=cuda_device)[:, None]).to(dtype)
+    slopes = 2.0 ** (-6 - torch.arange(heads, device=cuda_device).float()) if options.pop('bias', False) else None
+    prefix = [m - n // 2 for n, m in docs] if options.pop('prefix', False) else None
+    kernel, splits = _plan(q_off[-1], k_off[-1], len(docs), heads, kv_heads, d)
+    assert kernel == ROWS and above < splits <= most
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               prefix=None if prefix is None else _i32(prefix, cuda_device), slopes=slopes, **options)
+    _assert_close(got, *_reference(q, k, v, heads, kv_heads, q_off, k_off, prefix=prefix, slopes=slopes, **options))
+    assert bool((got[q_off[-2]:] == 0).all())
+
+
+@pytest.mark.parametrize('poison', [math.nan, math.inf])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('case', [0, 2])
+def test_rows_over_long_keys_last_values_not_finite(cuda_device, case, dtype, poison):
+    """A value at the last key that is not finite reaches the rows that see it: their split is taken again key by key
+    and joined with the other splits' sums."""
+    from musc_b200 import ops
+    docs, heads, kv_heads, d, (above, most) = LONG[case]
+    q_off, k_off = _starts([n for n, _ in docs]), _starts([m for _, m in docs])
+    kernel, splits = _plan(q_off[-1], k_off[-1], len(docs), heads, kv_heads, d)
+    assert kernel == ROWS and above < splits <= most
+    q, k, v = _random_qkv(cuda_device, q_off[-1], k_off[-1], heads, kv_heads, d, dtype, 220 + case, False)
+    clean = v.clone()
+    v[k_off[1] - 2, 5] = poison                               # seen by the last two rows of the first document
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               causal=True)
+    want, tol = _reference(q, k, clean, heads, kv_heads, q_off, k_off, causal=True)
+    hit = torch.zeros(got.shape, dtype=torch.bool, device=cuda_device)
+    hit[q_off[1] - 2:q_off[1], [h * d + 5 for h in range(heads // kv_heads)]] = True
+    assert not bool(got[hit].isfinite().any())
+    others = ~hit
+    others[q_off[1] - 2:q_off[1]] = False                     # (their bound would need the poisoned row's other values)
+    _assert_close(got[others], want[others], tol[others])
+    assert bool(got[~hit].isfinite().all())
+
+
+@pytest.mark.parametrize('kernel,n_q,n_k,heads,d', [(ROWS, 1, 100_000, 2, 64), (ROWS, 2, 60_000, 8, 128), (ROWS, 2, 3000, 4, 64),
+                                                    (TILES, 300, 9000, 4, 64), (TILES, 300, 500, 96, 128)])
+def test_keys_of_minus_infinity(cuda_device, kernel, n_q, n_k, heads, d):
+    """Visible scores of -infinity weigh nothing, in the middle of a split or in all of one; a row that has no other
+    score is 0 / 0."""
+    from musc_b200 import ops
+    q, k, v = _random_qkv(cuda_device, n_q, n_k, heads, 1, d, torch.bfloat16, 61, False)
+    q[:, ::d] = 1.0
+    first = n_k * 3 // 5
+    k[:first, 0] = -math.inf
+    assert _plan(n_q, n_k, 1, heads, 1, d)[0] == kernel
+    offsets = dict(offsets=_i32([0, n_q], cuda_device), kv_offsets=_i32([0, n_k], cuda_device))
+    got = ops.attention_masked(q, k, v, heads, 1, **offsets)
+    _assert_close(got, *_reference(q, k[first:], v[first:], heads, 1, [0, n_q], [0, n_k - first]))
+    k[:, 0] = -math.inf
+    assert bool(ops.attention_masked(q, k, v, heads, 1, **offsets).isnan().all())
+
+
+def test_splits_captured_and_on_other_streams(cuda_device):
+    """Calls that need a workspace, of both kernels: replays of their graphs and eager calls on two streams at once
+    give the eager result bit for bit."""
+    from musc_b200 import ops
+    calls = []
+    for kernel, above, n, keys, docs, heads, kv_heads, d in ((ROWS, 8, 8, 40_000, 2, 8, 1, 128), (TILES, 1, 300, 9000, 1, 4, 2, 64)):
+        got, splits = _plan(n, keys, docs, heads, kv_heads, d, True)
+        assert got == kernel and splits > above
+        q, k, v = _random_qkv(cuda_device, n, keys, heads, kv_heads, d, torch.float16, 62 + n, False)
+        kwargs = dict(offsets=_i32([n * i // docs for i in range(docs + 1)], cuda_device),
+                      kv_offsets=_i32([keys * i // docs for i in range(docs + 1)], cuda_device), causal=True)
+        calls.append(lambda q=q, k=k, v=v, h=heads, hk=kv_heads, kwargs=kwargs: ops.attention_masked(q, k, v, h, hk, **kwargs))
+    want = [c() for c in calls]
+    graphs = []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c()
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream(cuda_device) for _ in calls]
+    torch.cuda.synchronize()
+    eager = []
+    for i in range(6):
+        for j, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                graphs[(i + j) % 2][0].replay()   # each graph on both streams in turn, never on both at once
+                eager.append((j, c()))
+        torch.cuda.synchronize()
+    for (_, out), w in zip(graphs, want):
+        assert torch.equal(out, w)
+    for j, e in eager:
+        assert torch.equal(e, want[j])
+
+
+# ----------------------------------------------------------------------------- the tile kernel's lookup of documents
+def _lengths(kind):
+    g = torch.Generator().manual_seed(63)
+    if kind == '8 long':              # ending at and beside tile borders
+        return [256, 255, 257, 512, 1, 64, 65, 700]
+    if kind == '32':                  # the most documents that one warp looks up
+        return [70 + 5 * (i % 3) for i in range(30)] + [900, 0]
+    if kind == '33':
+        n = torch.randint(1, 90, (33,), generator=g)
+        n[20] = 1500
+    elif kind == '60':
+        n = torch.randint(0, 160, (60,), generator=g)
+        n[::9] += 300
+        n[5] = n[6] = 0
+    elif kind == '1024':              # the most that are looked up in shared memory: long, short and empty ones
+        n = torch.randint(0, 41, (1024,), generator=g)
+        n[torch.rand(1024, generator=g) < 0.15] += 420
+        n[torch.rand(1024, generator=g) < 0.1] = 0
+    elif kind == '1100':
+        n = torch.randint(8, 28, (1100,), generator=g)
+    else:                             # '40 short': tiles cut from the packed rows
+        n = torch.randint(0, 30, (40,), generator=g)
+    return n.tolist()
+
+
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('kind,heads,d', [('8 long', 16, 64), ('8 long', 8, 128), ('32', 16, 64), ('33', 16, 64), ('33', 8, 128),
+                                          ('60', 8, 64), ('1024', 2, 64), ('1100', 8, 64), ('40 short', 160, 64)])
+def test_tiles_of_many_documents(cuda_device, kind, heads, d, causal):
+    """Row tiles of many documents, packed rows before the first and behind the last one left alone."""
+    from musc_b200 import ops
+    lens = _lengths(kind)
+    off = [13 + o for o in _starts(lens)]
+    rows, kv_heads = off[-1] + 30, heads // 2
+    assert _plan(rows, rows, len(lens), heads, kv_heads, d, causal)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, rows, rows, heads, kv_heads, d, torch.bfloat16, 64, True)
+    out = torch.full_like(q, 3.0)
+    ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(off, cuda_device), causal=causal, out=out)
+    assert bool((out[:13] == 3).all()) and bool((out[off[-1]:] == 3).all())
+    first = 0
+    while first < len(lens):              # documents together that have up to 4000 rows
+        last = first + 1
+        while last < len(lens) and off[last + 1] - off[first] <= 4000:
+            last += 1
+        a, b = off[first], off[last]
+        part = [o - a for o in off[first:last + 1]]
+        _assert_heads(out[a:b], q[a:b], k[a:b], v[a:b], heads, kv_heads, part, part, causal=causal,
+                      rows=torch.ones(b - a, dtype=torch.bool, device=cuda_device))
+        first = last
+
+
+@pytest.mark.parametrize('length,heads', [(17, 512), (100, 64), (256, 16), (300, 16), (515, 16)])
+def test_tiles_of_batches_of_one_length(cuda_device, length, heads):
+    from musc_b200 import ops
+    kv_heads = heads // 2
+    assert _plan(5 * length, 5 * length, 5, heads, kv_heads, 64, True, (length, length))[0] == TILES
+    q, k, v = _random_qkv(cuda_device, 5 * length, 5 * length, heads, kv_heads, 64, torch.float16, 65, True)
+    view = lambda t: t.unflatten(0, (5, length))
+    got = ops.attention_masked(view(q), view(k), view(v), heads, kv_heads, causal=True, softcap=20.0)
+    off = _starts([length] * 5)
+    _assert_heads(got.flatten(0, 1), q, k, v, heads, kv_heads, off, off, causal=True, softcap=20.0)
+
+
+@pytest.mark.parametrize('documents', [3, 40])
+def test_tiles_disordered_offsets_stay_inside(cuda_device, documents):
+    """Offsets that fall, repeat or leave the tensors: results are undefined, accesses are not."""
+    from musc_b200 import ops
+    n, heads, kv_heads = 3000, 32, 16
+    assert _plan(n, n, documents, heads, kv_heads, 64, True)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, n, n, heads, kv_heads, 64, torch.float16, 66, True)
+    top = (1 << 31) - 1
+    g = torch.Generator().manual_seed(67)
+    anywhere = lambda lo, hi: torch.randint(lo, hi, (documents + 1,), generator=g).tolist()
+    sets = [(anywhere(0, n + 1), anywhere(0, n + 1)), (anywhere(-top, top), anywhere(-top, top)),
+            (sorted(anywhere(0, n), reverse=True), sorted(anywhere(0, n))), ([n] * (documents + 1), [0] * (documents + 1)),
+            ([-top - 1, top] * ((documents + 1) // 2) + [-5] * ((documents + 1) % 2), anywhere(0, n))]
+    for q_off, k_off in sets:
+        for causal in (False, True):
+            ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                                 kv_lengths=_i32(anywhere(-9, n)[1:], cuda_device), causal=causal)
+    torch.cuda.synchronize()
+    ops.check_device_error(cuda_device)
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32([0, n], cuda_device))
+    _assert_heads(got, q, k, v, heads, kv_heads, [0, n], [0, n])
+
+
+@pytest.mark.parametrize('heads,d', [(64, 64), (16, 128)])
+def test_tiles_key_offsets_past_the_tensor(cuda_device, heads, d):
+    from musc_b200 import ops
+    n, kv_heads = 500, heads // 2
+    assert _plan(n, 600, 1, heads, kv_heads, d)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, n, 600, heads, kv_heads, d, torch.float16, 68, False)
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32([0, n], cuda_device),
+                               kv_offsets=_i32([-50, 100_000], cuda_device), kv_lengths=_i32([1 << 30], cuda_device))
+    _assert_heads(got, q, k, v, heads, kv_heads, [0, n], [0, 600])
+
+
+# ----------------------------------------------------------------------------- the tile kernel's masks and scores
+@pytest.mark.parametrize('d,dtype', [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize('poison', [math.nan, math.inf, -math.inf])
+def test_tiles_masked_values_do_not_leak(cuda_device, poison, d, dtype):
+    """Keys and values that a row does not see may hold anything: later tokens of its own document, other
+    documents in the same tile, the type's lowest value in scores."""
+    from musc_b200 import ops
+    heads, lens = 160, [150, 30, 200, 9]
+    off = _starts(lens)
+    assert _plan(off[-1], off[-1], 4, heads, heads, d, True)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, off[-1], off[-1], heads, heads, d, dtype, 69, False)
+    late = [off[1] - 1, off[3] - 2]            # the last key of one document, the last but one of another
+    k[late] = torch.finfo(dtype).min
+    v[late] = poison
+    clean_k, clean_v = k.clone(), v.clone()
+    clean_k[late], clean_v[late] = 0, 0
+    got = ops.attention_masked(q, k, v, heads, offsets=_i32(off, cuda_device), causal=True)
+    clean = torch.ones(off[-1], dtype=torch.bool, device=cuda_device)
+    clean[off[1] - 1], clean[off[3] - 2:off[3]] = False, False
+    _assert_heads(got, q, clean_k, clean_v, heads, heads, off, off, causal=True, rows=clean)
+    # whole documents: only the poisoned ones are touched
+    got = ops.attention_masked(q, k, v, heads, offsets=_i32(off, cuda_device))
+    clean[:off[1]], clean[off[2]:off[3]] = False, False
+    _assert_heads(got, q, clean_k, clean_v, heads, heads, off, off, rows=clean)
+
+
+def test_tiles_visible_nan_and_infinity(cuda_device):
+    """A value that a row does see reaches it."""
+    from musc_b200 import ops
+    heads = 128
+    assert _plan(300, 300, 1, heads, heads, 64, True)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, 300, 300, heads, heads, 64, torch.float16, 70, False)
+    k = k * 0.1
+    v[280, 3::64], v[40, 5::64] = math.nan, math.inf
+    got = ops.attention_masked(q, k, v, heads, offsets=_i32([0, 300], cuda_device), causal=True)
+    assert torch.isnan(got[280:, 3::64]).all() and torch.isfinite(got[:280, 3::64]).all()
+    assert torch.isinf(got[40:, 5::64]).all() and torch.isfinite(got[:40, 5::64]).all()
+    q[7] = math.nan
+    got = ops.attention_masked(q, k, v, heads, offsets=_i32([0, 300], cuda_device), causal=True)
+    assert torch.isnan(got[7]).all() and torch.isfinite(got[:7]).all() and torch.isfinite(got[8:40]).all()
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_tiles_leave_rows_outside_documents(cuda_device, d):
+    """Rows outside every document are not written: one document, and tiles that documents begin themselves."""
+    from musc_b200 import ops
+    heads = 64
+    for lens in ([400], [300, 0, 290], [33] * 12):
+        off = [10 + o for o in _starts(lens)]
+        rows = off[-1] + 10
+        assert _plan(rows, rows, len(lens), heads, heads, d)[0] == TILES
+        q, k, v = _random_qkv(cuda_device, rows, rows, heads, heads, d, torch.float16, 71, True)
+        out = torch.full((rows, heads * d), 7.0, dtype=torch.float16, device=cuda_device)
+        ops.attention_masked(q, k, v, heads, offsets=_i32(off, cuda_device), out=out)
+        assert bool((out[:10] == 7).all()) and bool((out[off[-1]:] == 7).all())
+        _assert_heads(out, q, k, v, heads, heads, off, off)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('causal', [False, True])
+def test_tiles_cache_slots_ignore_what_lies_behind(cuda_device, causal, d):
+    """Key slots used to differing lengths: what lies behind a slot's keys changes nothing, bit for bit."""
+    from musc_b200 import ops
+    n_q, heads, kv_heads, slot, lengths = 300, 32, 16, 333, [333, 301, 0, 128, 300]
+    docs = len(lengths)
+    assert _plan(docs * n_q, docs * slot, docs, heads, kv_heads, d, causal)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, docs * n_q, docs * slot, heads, kv_heads, d, torch.bfloat16, 72, False)
+    q_off, k_off = _starts([n_q] * docs), _starts([slot] * docs)
+    results = []
+    for fill in (0.0, math.nan, math.inf):
+        for i, n in enumerate(lengths):
+            k[i * slot + n:(i + 1) * slot] = fill
+            v[i * slot + n:(i + 1) * slot] = -fill
+        results.append(ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device),
+                                            kv_offsets=_i32(k_off, cuda_device), kv_lengths=_i32(lengths, cuda_device),
+                                            causal=causal))
+        if fill == 0.0:
+            _assert_heads(results[0], q, k, v, heads, kv_heads, q_off, k_off, k_len=lengths, causal=causal)
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('softcap', [0.01, 3.0, 1e4, 1e7])
+def test_tiles_cap_far_from_the_scores(cuda_device, softcap, d):
+    """As the test of few heads: the rounding of P and of the result on the capped scores' own average, a dot product off
+    by (d + 8) 2^-24 of its terms' magnitudes, and 2^-20 of min(|z|, cap)."""
+    from musc_b200 import ops
+    n_q, n_k, heads = 200, 700, 64
+    assert _plan(n_q, n_k, 1, heads, heads, d)[0] == TILES
+    q, k, v = _random_qkv(cuda_device, n_q, n_k, heads, heads, d, torch.float16, 73, False)
+    q = q * 3
+    got = ops.attention_masked(q, k, v, heads, softcap=softcap, offsets=_i32([0, n_q], cuda_device),
+                               kv_offsets=_i32([0, n_k], cuda_device))
+    for h in (0, heads - 1):
+        qh, kh, vh = (_of_heads(t, d, h, 1) for t in (q, k, v))
+        want, _ = _reference(qh, kh, vh, 1, 1, [0, n_q], [0, n_k], softcap=softcap)
+        mean, _ = _reference(qh, kh, vh.abs(), 1, 1, [0, n_q], [0, n_k], softcap=softcap)
+        size = float((qh.double().abs() @ kh.double().abs().T).max()) * d ** -0.5
+        top = float((qh.double() @ kh.double().T).abs().max()) * d ** -0.5
+        tol = 2.0 ** -11 * (mean + want.abs()) * (1 + 2.0 ** -6) + 2.0 ** -24
+        tol = tol + 2 * mean * ((d + 8) * 2.0 ** -24 * size + 2.0 ** -18 + min(top, softcap) * 2.0 ** -20)
+        _assert_close(_of_heads(got, d, h, 1), want, tol)
