@@ -450,6 +450,12 @@ def rscin(image_scores: torch.Tensor, cls_tokens: torch.Tensor | None,
 
 
 # --------------------------------------------------------------------------- attention
+def _written(*tensors: torch.Tensor | None) -> None:
+    """Tells autograd of the caller's tensors that a kernel has written: a backward pass that still needs what
+    one of them held then raises instead of using what it holds now."""
+    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+
+
 def add_layernorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor,
                   eps: float = 1e-5, out_dtype: torch.dtype = torch.float16,
                   out: torch.Tensor | None = None) -> torch.Tensor:
@@ -466,6 +472,7 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Ten
             raise ValueError('add_layernorm: delta must be a contiguous fp16/bf16 tensor of x\'s shape')
     if out_dtype not in (torch.float16, torch.bfloat16):
         raise ValueError('add_layernorm: out_dtype must be float16 or bfloat16')
+    given = out
     if out is None:
         out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
     w, b = weight.contiguous(), bias.contiguous()
@@ -475,6 +482,7 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Ten
                                                 _ptr(w), _ptr(b), float(eps), _ptr(out), _DTYPES[out_dtype], rows, c,
                                                 _stream(dev))
         _lib.check(st, 'musc_b200_add_layernorm')
+    _written(x if delta is not None else None, given)
     return out
 
 
@@ -497,6 +505,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
     for t in (q, k, v):
         if t.stride(2) != 1 or t.stride(0) != length * t.stride(1) or t.stride(1) != q.stride(1):
             raise ValueError('attention: q, k, v must be token-major with one common row stride')
+    given = out
     if out is None:
         out = torch.empty(b, length, width, dtype=q.dtype, device=q.device)
     scale = head_dim ** -0.5 if scale is None else scale
@@ -507,6 +516,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
                                                 head_dim, q.stride(1), out.stride(1), float(scale),
                                                 _stream(dev))
         _lib.check(st, 'musc_b200_attention_fwd')
+    _written(given)
     return out
 
 
@@ -624,6 +634,7 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     _, v_stride, v_pitch = _token_rows(what, 'v', v)
     if q.ndim == 3 and (q_pitch != q.shape[1] or v_pitch != kv_pitch):
         raise ValueError('attention_masked: batch items of q must follow each other, those of k and v lie equally far apart')
+    given = out
     if out is None:
         out, out_stride = _packed_like(q), heads * head_dim
     else:
@@ -646,6 +657,8 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
         st = lib.musc_b200_masked_attention(ctypes.byref(args), _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_masked_attention')
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -732,6 +745,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
             frequencies.shape[0], adjacent, _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_rotary')
+    if out is not None:
+        _written(q_out, k_out)
     return q_out, k_out
 
 
@@ -767,6 +782,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
         raise ValueError('add_rmsnorm: out_dtype must be float32, float16, bfloat16 or float8_e4m3fn')
     if group not in (0, 32, 64, 128, 256) or (group and not eight):
         raise ValueError('add_rmsnorm: group must be 0, or 32, 64, 128 or 256 for a float8_e4m3fn output')
+    given = x if delta is not None else None, out, scales
     if out is None:
         out = _packed_like(x, out_dtype)
     if out.shape != x.shape or out.dtype != out_dtype:
@@ -796,6 +812,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
             rows, c, strides[0], strides[1], strides[2], _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_add_rmsnorm')
+    _written(*given)
     return (out, scales) if eight else out
 
 

@@ -384,3 +384,58 @@ def test_tiles_cap_far_from_the_scores(cuda_device, softcap, d):
         tol = 2.0 ** -11 * (mean + want.abs()) * (1 + 2.0 ** -6) + 2.0 ** -24
         tol = tol + 2 * mean * ((d + 8) * 2.0 ** -24 * size + 2.0 ** -18 + min(top, softcap) * 2.0 ** -20)
         _assert_close(_of_heads(got, d, h, 1), want, tol)
+
+
+# ----------------------------------------------------------------------------- writes that autograd has to know of
+def _block_writes(dev):
+    """(name, call, tensor that it writes): every block operator that writes a tensor of the caller's."""
+    from musc_b200 import ops
+    half = lambda *shape: torch.randn(*shape, device=dev).half()
+    qkv = [half(2, 40, 128) for _ in range(3)]
+    rows = [half(40, 128) for _ in range(3)]
+    off = _i32([0, 40], dev)
+    f, a = ops.rotary_frequencies([32], device=dev)
+    pos = torch.arange(40, dtype=torch.int32, device=dev)[:, None]
+    x, h, delta, w = torch.randn(40, 128, device=dev), half(40, 128), half(40, 128), torch.ones(128, device=dev)
+    scales, eight = torch.zeros(40, 1, device=dev), torch.zeros(40, 128, device=dev).to(torch.float8_e4m3fn)
+    o3, o2 = half(2, 40, 128), half(40, 128)
+    return [
+        ('attention out', lambda: ops.attention(*qkv, 2, out=o3), o3),
+        ('attention_masked out', lambda: ops.attention_masked(*rows, 2, offsets=off, out=o2), o2),
+        ('rotary q', lambda: ops.rotary(rows[0], rows[1], pos, f, a, 2, out=(rows[0], rows[1])), rows[0]),
+        ('rotary k', lambda: ops.rotary(rows[0], rows[1], pos, f, a, 2, out=(rows[0], rows[1])), rows[1]),
+        ('add_layernorm x', lambda: ops.add_layernorm(x, delta, w, w), x),
+        ('add_layernorm out', lambda: ops.add_layernorm(x, None, w, w, out=o2), o2),
+        ('add_rmsnorm x', lambda: ops.add_rmsnorm(x, delta, w), x),
+        ('add_rmsnorm 16-bit x', lambda: ops.add_rmsnorm(h, delta, w), h),
+        ('add_rmsnorm out', lambda: ops.add_rmsnorm(x, None, w, out=o2), o2),
+        ('add_rmsnorm scales', lambda: ops.add_rmsnorm(x, None, w, out_dtype=torch.float8_e4m3fn, out=eight, scales=scales), scales),
+    ]
+
+
+@pytest.mark.parametrize('which', range(10))
+def test_writes_reach_autograd(cuda_device, which):
+    """A tensor that a backward pass still needs and a block operator then overwrites is noticed by it, also where
+    the operator was given a view."""
+    name, call, written = _block_writes(cuda_device)[which]
+    factor = torch.ones_like(written).requires_grad_()
+    y = (factor * written).sum()                              # keeps `written` for the gradient of `factor`
+    with torch.no_grad():
+        call()
+    with pytest.raises(RuntimeError, match='inplace'):
+        y.backward()
+    with torch.inference_mode():
+        _block_writes(cuda_device)[which][1]()                # tensors without a version
+
+
+def test_reads_leave_versions_alone(cuda_device):
+    from musc_b200 import ops
+    x, w = torch.randn(40, 128, device=cuda_device), torch.ones(128, device=cuda_device)
+    q = torch.randn(40, 128, device=cuda_device).half()
+    versions = x._version, q._version
+    ops.add_rmsnorm(x, None, w)
+    ops.add_layernorm(x, None, w, w)
+    ops.attention_masked(q, q, q, 2, offsets=_i32([0, 40], cuda_device))
+    f, a = ops.rotary_frequencies([32], device=cuda_device)
+    ops.rotary(q, q, torch.zeros(40, 1, dtype=torch.int32, device=cuda_device), f, a, 2)
+    assert (x._version, q._version) == versions
