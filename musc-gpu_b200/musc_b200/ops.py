@@ -14,6 +14,7 @@ import math
 from typing import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -521,11 +522,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, sca
 
 
 def _forward_only(what: str, *tensors: torch.Tensor | None) -> None:
-    """These operators have no backward pass: refuse inputs whose gradient would be lost."""
+    """These operators have no backward pass and no forward-mode one: refuse inputs (and given outputs) whose
+    gradient or tangent would be lost."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f'{what}: no gradient is computed; call it under torch.no_grad() or detach the inputs')
+    if forward_ad._current_level >= 0:  # within a dual_level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f'{what}: no tangent is computed; call it with the primal tensors')
 
 
 def _on_device(what: str, device: torch.device, **tensors: torch.Tensor | None) -> None:
@@ -601,7 +607,7 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     """
     what = 'attention_masked'
     _require_cuda(q, what)
-    _forward_only(what, q, k, v, slopes)
+    _forward_only(what, q, k, v, slopes, out)
     dev = q.device
     _on_device(what, dev, k=k, v=v, offsets=offsets, kv_offsets=kv_offsets, kv_lengths=kv_lengths, prefix=prefix,
                slopes=slopes, out=out)
@@ -697,7 +703,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     """
     what = 'rotary'
     _require_cuda(q, what)
-    _forward_only(what, q, k, positions, frequencies)
+    _forward_only(what, q, k, positions, frequencies, *(out or ()))
     dev = q.device
     _on_device(what, dev, k=k, positions=positions, frequencies=frequencies, axis=axis)
     if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
@@ -766,7 +772,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
     """
     what = 'add_rmsnorm'
     _require_cuda(x, what)
-    _forward_only(what, x, delta, weight)
+    _forward_only(what, x, delta, weight, out, scales)
     dev = x.device
     _on_device(what, dev, delta=delta, weight=weight, out=out, scales=scales)
     if x.ndim < 1 or x.dtype not in _DTYPES:

@@ -204,3 +204,18 @@ def test_attention_plan_of_long_contexts(head_dim):
             tiles, splits = _plan(q_rows=1, **sizes)
             assert tiles == 0 and splits > 32
             assert _plan(q_rows=256, **dict(sizes, heads=2, kv_heads=1)) == (1, 32)
+
+
+def test_forward_only_refuses_gradients_and_tangents():
+    from torch.autograd import forward_ad
+    x, asks = torch.ones(3), torch.ones(3, requires_grad=True)
+    ops._forward_only('op', x, None)
+    with pytest.raises(ValueError, match='gradient'):
+        ops._forward_only('op', x, None, asks)
+    with torch.no_grad():
+        ops._forward_only('op', asks)
+    with forward_ad.dual_level():
+        ops._forward_only('op', x, None)
+        for enabled in (True, False):
+            with torch.set_grad_enabled(enabled), pytest.raises(ValueError, match='tangent'):
+                ops._forward_only('op', None, forward_ad.make_dual(x, x))

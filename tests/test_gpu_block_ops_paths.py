@@ -439,3 +439,29 @@ def test_reads_leave_versions_alone(cuda_device):
     f, a = ops.rotary_frequencies([32], device=cuda_device)
     ops.rotary(q, q, torch.zeros(40, 1, dtype=torch.int32, device=cuda_device), f, a, 2)
     assert (x._version, q._version) == versions
+
+
+def test_gradients_and_tangents_are_refused(cuda_device):
+    """Inputs and given outputs that ask for a gradient, and inputs with a tangent of forward mode."""
+    from torch.autograd import forward_ad
+
+    from musc_b200 import ops
+    q = torch.randn(40, 128, device=cuda_device).half()
+    x, w = torch.randn(40, 128, device=cuda_device), torch.ones(128, device=cuda_device)
+    off, pos = _i32([0, 40], cuda_device), torch.zeros(40, 1, dtype=torch.int32, device=cuda_device)
+    f, a = ops.rotary_frequencies([32], device=cuda_device)
+    asks = lambda t: t.clone().requires_grad_()
+    scales = torch.zeros(40, 1, device=cuda_device)
+    for call in (lambda t: ops.attention_masked(q, q, q, 2, offsets=off, out=t(q)),
+                 lambda t: ops.attention_masked(q, t(q), q, 2, offsets=off),
+                 lambda t: ops.rotary(q, q, pos, f, a, 2, out=(t(q), q.clone())),
+                 lambda t: ops.rotary(q, None, pos.float(), t(f), a, 2),
+                 lambda t: ops.add_rmsnorm(t(x), None, w), lambda t: ops.add_rmsnorm(x, t(q), w),
+                 lambda t: ops.add_rmsnorm(x, None, w, out=t(q)),
+                 lambda t: ops.add_rmsnorm(x, None, w, out_dtype=torch.float8_e4m3fn, scales=t(scales))):
+        with pytest.raises(ValueError, match='gradient'):
+            call(asks)
+        with torch.no_grad():
+            call(asks)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match='tangent'):
+            call(lambda t: forward_ad.make_dual(t.clone(), torch.ones_like(t)))
