@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_block_ops import _assert_close, _i32, _of_heads, _random_qkv, _reference, _starts
+from test_gpu_block_ops import _assert_close, _i32, _normed, _of_heads, _random_qkv, _reference, _starts
 
 pytestmark = pytest.mark.gpu
 
@@ -465,3 +465,80 @@ def test_gradients_and_tangents_are_refused(cuda_device):
             call(asks)
         with forward_ad.dual_level(), pytest.raises(ValueError, match='tangent'):
             call(lambda t: forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+
+
+# ----------------------------------------------------------------------------- the norm's walk over rows
+# Rows enough that every CTA takes at least three (a warp's or its own) on 148 SMs with a last step that some leave out.
+WALKS = [(60_001, 64), (60_001, 100), (20_003, 1480), (9001, 1481), (5003, 5000), (5003, 5003), (2501, 12_296), (2000, 20_001),
+         (2003, 16_384), (1999, 32_768), (60_001, 1024)]
+
+
+def _walk_inputs(rows, c, dev, x_dtype=torch.float32):
+    g = torch.Generator(device=dev).manual_seed(rows + c)
+    x = torch.randn(rows, c, generator=g, device=dev) * torch.exp(2 * torch.randn(rows, 1, generator=g, device=dev))
+    delta = (0.5 * torch.randn(rows, c, generator=g, device=dev)).to(torch.bfloat16)
+    w = 1 + 0.2 * torch.randn(c, generator=g, device=dev)
+    return x.to(x_dtype), delta, w
+
+
+@pytest.mark.parametrize('x_dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('rows,c', WALKS)
+def test_norm_walk_over_rows(cuda_device, rows, c, x_dtype):
+    from musc_b200 import ops
+    x, delta, w = _walk_inputs(rows, c, cuda_device, x_dtype)
+    want_x = (x.float() + delta.float()).to(x_dtype)
+    want = _normed(x, delta, w, 1e-6)
+    got = ops.add_rmsnorm(x, delta, w, 1e-6, torch.float16)
+    assert torch.equal(x, want_x)
+    _assert_close(got, want, want.abs() * (2.0 ** -18 + 2.0 ** -11) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize('group', [0, 32, 128, 256])
+@pytest.mark.parametrize('rows,c', WALKS)
+def test_norm_walk_over_rows_eight_bits(cuda_device, rows, c, group):
+    from musc_b200 import ops
+    x, delta, w = _walk_inputs(rows, c, cuda_device)
+    want = _normed(x, delta, w, 1e-6)
+    values, scales = ops.add_rmsnorm(x, delta, w, 1e-6, torch.float8_e4m3fn, group=group)
+    size = group or c
+    n = -(-c // size)
+    top = torch.nn.functional.pad(want, (0, n * size - c)).view(rows, n, size).abs().amax(-1) / 448
+    _assert_close(scales, top, top * 2.0 ** -17 + 2.0 ** -125)
+    want /= scales.double().repeat_interleave(size, 1)[:, :c]
+    _assert_close(values.float(), want, want.abs() * (2.0 ** -4 + 2.0 ** -16) + 2.0 ** -10)
+
+
+# ----------------------------------------------------------------------------- given outputs with rows a stride apart
+@pytest.mark.parametrize('kernel,above,n_q,n_k,docs,heads,kv_heads,d', [
+    (ROWS, 0, 9, 700, 1, 8, 8, 64), (ROWS, 1, 4, 3000, 1, 4, 2, 64), (ROWS, 8, 8, 40_000, 2, 8, 1, 128),
+    (TILES, 0, 500, 500, 1, 64, 64, 64), (TILES, 1, 300, 9000, 1, 4, 2, 64)])
+def test_attention_into_columns(cuda_device, kernel, above, n_q, n_k, docs, heads, kv_heads, d):
+    """q, k, v and out as columns of wider buffers, each with its own row stride; the columns beside out stay."""
+    from musc_b200 import ops
+    got, splits = _plan(n_q, n_k, docs, heads, kv_heads, d, True)
+    assert got == kernel and splits > above
+    g = torch.Generator(device=cuda_device).manual_seed(74)
+    rand = lambda rows, width, extra: torch.randn(rows, width + extra, generator=g, device=cuda_device).half()
+    q, k, v = rand(n_q, heads * d, 24)[:, 16:-8], rand(n_k, kv_heads * d, 8)[:, 8:], rand(n_k, kv_heads * d, 72)[:, :-72]
+    buf = torch.full((n_q, heads * d + 40), 5.0, dtype=torch.float16, device=cuda_device)
+    q_off, k_off = [n_q * i // docs for i in range(docs + 1)], [n_k * i // docs for i in range(docs + 1)]
+    out = buf[:, 8:-32]
+    assert ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                                causal=True, out=out) is out
+    assert bool((buf[:, :8] == 5).all()) and bool((buf[:, -32:] == 5).all())
+    _assert_heads(out, q, k, v, heads, kv_heads, q_off, k_off, causal=True)
+
+
+@pytest.mark.parametrize('kernel,n_q,n_k,docs,heads,kv_heads,d', [
+    (ROWS, 4, 5480, 4, 16, 16, 64), (ROWS, 8, 40_000, 2, 8, 1, 128), (ROWS, 9, 900, 3, 8, 2, 128), (TILES, 900, 900, 3, 64, 64, 64),
+    (TILES, 300, 9000, 1, 4, 2, 64)])
+def test_attention_repeats_itself(cuda_device, kernel, n_q, n_k, docs, heads, kv_heads, d):
+    """The same call gives the same bits: no sum depends on the order in which CTAs run."""
+    from musc_b200 import ops
+    assert _plan(n_q, n_k, docs, heads, kv_heads, d, True)[0] == kernel
+    q, k, v = _random_qkv(cuda_device, n_q, n_k, heads, kv_heads, d, torch.bfloat16, 75, False)
+    offsets = dict(offsets=_i32([n_q * i // docs for i in range(docs + 1)], cuda_device),
+                   kv_offsets=_i32([n_k * i // docs for i in range(docs + 1)], cuda_device))
+    first = ops.attention_masked(q, k, v, heads, kv_heads, causal=True, softcap=30.0, **offsets)
+    for _ in range(20):
+        assert torch.equal(ops.attention_masked(q, k, v, heads, kv_heads, causal=True, softcap=30.0, **offsets), first)
