@@ -83,16 +83,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <bool FP16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (FP16) {
-    __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&t);
-  }
-  __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&t);
-}
-
 // Eight finished dimensions of a head.
 template <bool FP16>
 __device__ __forceinline__ void store_eight(const Params& p, long long row, int column, const float (&acc)[8], float inv) {

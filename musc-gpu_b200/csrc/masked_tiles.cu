@@ -139,16 +139,6 @@ template <int D, bool FP16> constexpr uint32_t idesc_pv() {
   return tc::idesc_f16(BQ, D, FP16 ? 0 : 1) | (1u << 16);  // B (V) MN-major
 }
 
-template <bool FP16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (FP16) {
-    __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&t);
-  }
-  __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&t);
-}
-
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
