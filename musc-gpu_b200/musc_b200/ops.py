@@ -451,10 +451,11 @@ def rscin(image_scores: torch.Tensor, cls_tokens: torch.Tensor | None,
 
 
 # --------------------------------------------------------------------------- attention
-def _written(*tensors: torch.Tensor | None) -> None:
-    """Tells autograd of the caller's tensors that a kernel has written: a backward pass that still needs what
-    one of them held then raises instead of using what it holds now."""
-    torch.autograd.graph.increment_version([t for t in tensors if t is not None])
+def _written(t: torch.Tensor | None) -> None:
+    """Tells autograd of a tensor of the caller's that a kernel has written: a backward pass that still needs
+    what it held then raises instead of using what it holds now."""
+    if t is not None:
+        torch.autograd.graph.increment_version(t)
 
 
 def add_layernorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tensor, bias: torch.Tensor,
@@ -483,7 +484,9 @@ def add_layernorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Ten
                                                 _ptr(w), _ptr(b), float(eps), _ptr(out), _DTYPES[out_dtype], rows, c,
                                                 _stream(dev))
         _lib.check(st, 'musc_b200_add_layernorm')
-    _written(x if delta is not None else None, given)
+    if delta is not None:
+        _written(x)
+    _written(given)
     return out
 
 
@@ -663,8 +666,7 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
         st = lib.musc_b200_masked_attention(ctypes.byref(args), _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_masked_attention')
-    if given is not None:
-        _written(given)
+    _written(given)
     return out
 
 
@@ -752,7 +754,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_rotary')
     if out is not None:
-        _written(q_out, k_out)
+        _written(q_out)
+        _written(k_out)
     return q_out, k_out
 
 
@@ -788,7 +791,7 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
         raise ValueError('add_rmsnorm: out_dtype must be float32, float16, bfloat16 or float8_e4m3fn')
     if group not in (0, 32, 64, 128, 256) or (group and not eight):
         raise ValueError('add_rmsnorm: group must be 0, or 32, 64, 128 or 256 for a float8_e4m3fn output')
-    given = x if delta is not None else None, out, scales
+    given, given_scales = out, scales
     if out is None:
         out = _packed_like(x, out_dtype)
     if out.shape != x.shape or out.dtype != out_dtype:
@@ -818,7 +821,10 @@ def add_rmsnorm(x: torch.Tensor, delta: torch.Tensor | None, weight: torch.Tenso
             rows, c, strides[0], strides[1], strides[2], _raw_stream(dev))
         if st != _lib.OK:
             _lib.check(st, 'musc_b200_add_rmsnorm')
-    _written(*given)
+    if delta is not None:
+        _written(x)
+    _written(given)
+    _written(given_scales)
     return (out, scales) if eight else out
 
 
