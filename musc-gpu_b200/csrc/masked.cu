@@ -85,14 +85,17 @@ long long mean_keys(const musc_b200_masked_attention_args& a) {
 }
 
 // Whether the tile kernel is the faster one, by estimates in microseconds for mean documents that were
-// fitted to 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys): 0.6 % over the faster of
-// both in the mean, at most 1.39 times; on 110 others 1.0 % and 1.51 times.  A CTA of the row kernel takes up
+// fitted to 110 shapes (1 to 490 documents of 2 to 1865 rows over 2 to 14000 keys).  Over the faster of both:
+// 0.5 % in the mean, at most 1.42 times; on 110 others 0.6 % and 1.45 times.  A CTA of the row kernel takes up
 // to 16 rows x heads of one document and key head; one of the tile kernel takes 256 rows of one head over the
 // keys of all documents in them, and starts slowly.
-//   61 rows of 8 documents, 4 heads x 128: rows 6.7 us, tiles 16.4
-//   1020 rows of 129 documents, 1 head x 64: rows 267 us, tiles 100
-//   12 rows of 403 documents, 16 heads x 128: rows 113 us, tiles 57
-//   8 rows over 20000 keys of 2 documents, 8 heads on one key head x 128: rows 26 us, tiles 42
+//   43 documents of 3 rows over 366 keys, 16/2 heads x 64: rows 8.6 us, tiles 211
+//   129 documents of 1020 rows, 1 head x 64: rows 268 us, tiles 101
+//   403 documents of 12 rows, 16 heads x 128: rows 116 us, tiles 58
+//   2 documents of 4 rows over 20000 keys, 8/1 heads x 128: rows 25 us, tiles 52
+// Means: a call of one long document and many short ones takes one kernel for both.  One of 4096 rows with 63 of
+// 1 row over 4096 keys each, 32/8 heads x 128, takes tiles, whose 63 single rows share a row tile that walks all
+// their keys: 4.5 ms, 0.35 in two calls.
 // A row tile of a head has at most MAX_TILE_SPLITS CTAs, so fewer than five of them leave SMs idle.  On 103 shapes
 // of 1 to 300 rows, 1 to 8 heads and 8000 to 1000000 keys: 5 % over the faster of both in the mean, at most
 // 1.46 times (without that bound 15 % and 2.45 times).

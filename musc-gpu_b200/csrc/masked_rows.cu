@@ -3,7 +3,7 @@
 //
 // Keys and values are read once for a block's rows and all query heads of their group, and nothing
 // else is large: memory bounds it.  The group's heads, for as many consecutive rows of a document as fit
-// (5 rows over 2985 keys of 20 requests in 16.8 us, 34 when each row read the keys for itself), are the
+// (5 rows over 2985 keys of 20 requests, 8/2 heads x 128, in 24.5 us, 35 when each row read the keys for itself), are the
 // 16 rows of the tensor core's m16n8k16 products (a larger group takes several CTAs): S = Q K^T over 16
 // keys and the head dimension, then O += P V, at 2 x 16 x 16 x D operations per 64 D bytes far below
 // what the tensor cores give.  Each of the CTA's warps takes every WARPS-th run of 16 keys through a
@@ -432,11 +432,12 @@ int rows_together(int group, bool several) { return several ? std::max(1, HEADS 
 // A CTA takes its keys, 128 to start and 20 a row for the join, once for each wave of them; a split 20
 // more, the grid 130 for each fill of the GPU, and more splits than a cluster's eight a second launch
 // that reads them all.
-//   2 rows over 6390 keys of 7 requests, 56 units: 392 CTAs 25.1 us, 448 (444 are resident) 32.5
-//   553 keys of 12 requests, 24 units: in one split 10.6 us, in two 8.7, in five 6.8
-//   15 rows x heads over 450 keys, 56 units: 10.6 us in one, 11.5 in two, 18.2 in seven
-//   8 rows over 20000 keys of 2 requests, 8 units: 39 us in eight, 27 in sixteen
-//   one row over 60000 keys, 8 units: 52 us in sixteen, 49 in 32, 56 in 52
+// At D = 128, bf16, keys and values of three calls in turn:
+//   2 rows over 6390 keys of 7 requests, 8 key heads (56 units): 392 CTAs 35.0 us, 448 (444 are resident) 48.1
+//   1 row over 553 keys of 12 requests, 16/2 heads (24 units): in one split 9.7 us, in two 8.7, in five 7.6
+//   15 rows over 450 keys of 7 requests, 8 key heads (56 units): 11.2 us in one, 11.6 in two, 17.8 in seven
+//   4 rows over 20000 keys of 2 requests, 16/4 heads (8 units): 41.9 us in eight, 33.6 in sixteen
+//   1 row over 60000 keys, 8 key heads (8 units): 56 us in sixteen, 51 in 32, 58 in 52
 int rows_splits(long long units, long long keys, int rows, int head_dim) {
   const long long resident = 148LL * (head_dim == 64 ? RESIDENT<64> : RESIDENT<128>);
   int best = 1;

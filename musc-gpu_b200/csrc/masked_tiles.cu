@@ -4,8 +4,8 @@
 // One CTA per (256 query rows, head, split of the keys), 384 threads.  Its rows need not belong
 // to one document: every row carries its own key interval, and the CTA walks the union of its
 // documents' intervals in tiles of 64 keys, so short documents share a row tile; long ones begin
-// their own (one that holds two long documents' rows walks both their keys: 4 x 1370 tokens of 16
-// heads take 100 us, 170 when tiles are cut from the packed rows).
+// their own (one that holds two long documents' rows walks both their keys: nine images of 414 to
+// 932 tokens, 16 heads x 64, take 58 us, 71 when tiles are cut from the packed rows; 4 x 1370 tokens 83 and 87).
 //   warps 0-3, 4-7  softmax of query rows 0-127 and 128-255 (the two halves), one thread
 //                   per row: S out of tensor memory, cap, bias, mask, running maximum and
 //                   sum in 32 bits, P rounded to 16 bits into tensor memory beside S;
@@ -16,8 +16,9 @@
 // While one half's softmax runs, the tensor cores work for the other.  For 64 keys the exponentials
 // of both halves take 1024 cycles (16 a cycle and SM), the products 700 for D = 64 and 1350 for D = 128
 // (S of 128 x 64 runs at two thirds of the rate of 128 x 128, whose S would leave no tensor memory
-// for P beside it).  Measured at 8192 tokens of 16 heads, no mask, bf16: D = 128 509 us (1080 TF/s, 0.64
-// of the measured 1693), D = 64 493 us (557 TF/s); four waves of CTAs for 3.46 waves of work.  The
+// for P beside it).  Measured at 8192 tokens of 16 heads, no mask, bf16, calls apart: D = 128 509 us (1080 TF/s,
+// 0.64 of the measured 1693), D = 64 486 us (566 TF/s); four waves of CTAs for 3.46 waves of work.  (18 calls back to
+// back run at lower clocks: D = 128 556 us, D = 64 481.)  The
 // special-function unit is 60 % busy, the tensor pipe 29 % (D = 64, ncu): the rest is the softmax warps'
 // own chain, two of them a scheduler.  Tried and dropped, with times at D = 64 or 128: tiles of 128 keys with P over
 // S (548 us), a maximum of every tile before its exponentials (no gain from leaving it out by itself, but
@@ -861,9 +862,9 @@ int launch_form(const Params& p, cudaStream_t s) {
 }  // namespace
 
 // One wave of CTAs (148 SMs): a second one costs more than the finer division gives (2048 tokens of 16
-// heads in 37 us, with two waves 57).  With a causal mask the last rows' CTAs take twice the mean, and long
-// ones are divided for that: 8192 tokens of 4 heads in 78 us, in one piece 118; 2753 tokens of
-// 16 heads in 67 us, divided 78.
+// heads x 64 in 37 us, with two waves 57).  With a causal mask the last rows' CTAs take twice the mean, and long
+// ones are divided for that: 8192 tokens of 4 heads x 64 in 78 us, in one piece 120; 2753 tokens of
+// 16 heads x 128 in 53 us, divided 80.
 int tiles_splits(long long units, long long keys, bool causal) {
   units = std::max<long long>(units, 1);
   long long splits = std::min<long long>(148 / units, keys / 256);

@@ -607,6 +607,11 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     ``softcap * tanh(z / softcap)`` if ``softcap > 0``, less ``slopes[head] * distance`` with ``slopes``
     ``(heads,)`` fp32.  A row that sees no key gives zeros; rows outside every document are left as they
     are (of a fresh output: undefined).  Forward only.
+
+    One kernel and one split of the keys serve the whole call, by the documents' mean lengths: call long
+    prompts and many single tokens apart (4096 rows and 63 single rows over 4096 keys each, 32/8 heads x 128:
+    4.5 ms in one call, 0.35 in two).  A document's last bits may differ with what it is batched with; the
+    same call repeats itself bit for bit.
     """
     what = 'attention_masked'
     _require_cuda(q, what)
