@@ -382,7 +382,7 @@ int musc_b200_add_layernorm(float* x, const void* delta, int delta_dtype, const 
  * musc_b200_add_layernorm.  Per row (rows x_stride, delta_stride, out_stride
  * elements apart): h = x + delta in fp32 (delta NULL = no add), x = h rounded to
  * x_dtype (untouched without delta), y = h / sqrt(mean(h^2) + eps) * weight from
- * the unrounded h.  x and delta f32, f16 or bf16; weight [channels] f32.  out: y in
+ * the unrounded h (the sum of squares in fp32: |h| up to 2^56).  x and delta f32, f16 or bf16; weight [channels] f32.  out: y in
  * f32, f16 or bf16, or e4m3: out = y / scale rounded to nearest, with
  * scales [rows][ceil(channels / group)] fp32 = max |y| / 448 over the row (group
  * 0: one scale) or over each group of 32, 64, 128 or 256 columns (a row or

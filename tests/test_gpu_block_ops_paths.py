@@ -542,3 +542,93 @@ def test_attention_repeats_itself(cuda_device, kernel, n_q, n_k, docs, heads, kv
     first = ops.attention_masked(q, k, v, heads, kv_heads, causal=True, softcap=30.0, **offsets)
     for _ in range(20):
         assert torch.equal(ops.attention_masked(q, k, v, heads, kv_heads, causal=True, softcap=30.0, **offsets), first)
+
+
+# ----------------------------------------------------------------------------- far rows, many documents, many splits
+@pytest.mark.parametrize('kernel,n_q,n_k,heads,d', [(ROWS, 6, 40, 2, 64), (TILES, 300, 290, 160, 64)])
+def test_rows_whose_offsets_pass_32_bits(cuda_device, kernel, n_q, n_k, heads, d):
+    """Queries, keys, values and outputs 2^31 elements and more from their first row."""
+    from musc_b200 import ops
+    assert _plan(n_q, n_k, 1, heads, heads, d, True)[0] == kernel
+    size, width = (1 << 31) + (1 << 30), heads * d
+    buf, into = (torch.empty(size, dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    far = lambda t, of: of.as_strided(t.shape, ((size - width) // t.shape[0] // 8 * 8, 1))
+    q, k, v = _random_qkv(cuda_device, n_q, n_k, heads, heads, d, torch.bfloat16, 76, False)
+    offsets = dict(offsets=_i32([0, n_q], cuda_device), kv_offsets=_i32([0, n_k], cuda_device), causal=True)
+    for which in range(3):
+        given = [q, k, v]
+        given[which] = far(given[which], buf).copy_(given[which])
+        out = ops.attention_masked(*given, heads, out=far(q, into), **offsets)
+        _assert_heads(out.clone(), q, k, v, heads, heads, [0, n_q], [0, n_k], causal=True)
+
+
+@pytest.mark.parametrize('most', [1, 6])
+def test_rows_of_more_documents_than_a_warp_counts(cuda_device, most):
+    """Above 1024 documents their rows are searched for; documents of no rows and of no keys among them."""
+    from musc_b200 import ops
+    docs, heads, d = 2000, 4, 128
+    g = torch.Generator().manual_seed(77 + most)
+    q_lens, k_lens = (torch.randint(0, n + 1, (docs,), generator=g).tolist() for n in (most, 60))
+    q_off, k_off = [3 + o for o in _starts(q_lens)], _starts(k_lens)
+    rows = q_off[-1] + 3
+    assert _plan(rows, k_off[-1], docs, heads, 1, d, True)[0] == ROWS and (rows > docs) == (most > 1)
+    q, k, v = _random_qkv(cuda_device, rows, k_off[-1], heads, 1, d, torch.float16, 78, False)
+    out = torch.full_like(q, 4.0)
+    ops.attention_masked(q, k, v, heads, 1, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device), causal=True, out=out)
+    assert bool((out[:3] == 4).all()) and bool((out[-3:] == 4).all())
+    for first in range(0, docs, 250):
+        a, b, ka, kb = q_off[first], q_off[first + 250], k_off[first], k_off[first + 250]
+        want, tol = _reference(q[a:b], k[ka:kb], v[ka:kb], heads, 1, [o - a for o in q_off[first:first + 251]],
+                               [o - ka for o in k_off[first:first + 251]], causal=True)
+        _assert_close(out[a:b], want, tol)
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('poison', [0.0, math.nan])
+@pytest.mark.parametrize('n_q,n_k,docs,kv_heads,d', [(300, 60_000, 1, 1, 64), (500, 90_000, 2, 2, 128)])
+def test_tiles_over_long_keys_in_many_splits(cuda_device, n_q, n_k, docs, kv_heads, d, poison, dtype):
+    """The tile kernel's most splits, with maxima that differ from split to split; a NaN in a value that only the last
+    rows see stays with them."""
+    from musc_b200 import ops
+    heads = 2
+    assert _plan(n_q, n_k, docs, heads, kv_heads, d, True) == (TILES, 32)
+    q, k, v = _random_qkv(cuda_device, n_q, n_k, heads, kv_heads, d, dtype, 79, False)
+    k = (k.float() * torch.linspace(0.2, 2.0, n_k, device=cuda_device)[:, None]).to(dtype)
+    q_off, k_off = [n_q * i // docs for i in range(docs + 1)], [n_k * i // docs for i in range(docs + 1)]
+    clean = v.clone()
+    v[k_off[1] - 2, 5] += poison
+    got = ops.attention_masked(q, k, v, heads, kv_heads, offsets=_i32(q_off, cuda_device), kv_offsets=_i32(k_off, cuda_device),
+                               causal=True, softcap=20.0)
+    want, tol = _reference(q, k, clean, heads, kv_heads, q_off, k_off, causal=True, softcap=20.0)
+    hit = torch.zeros(got.shape, dtype=torch.bool, device=cuda_device)
+    if poison:
+        hit[q_off[1] - 2:q_off[1], [h * d + 5 for h in range(heads // kv_heads)]] = True
+        assert bool(got[hit].isnan().all())
+    _assert_close(got[~hit], want[~hit], tol[~hit])
+
+
+@pytest.mark.parametrize('c', [1024, 1001, 8192])
+def test_norm_and_rotary_of_far_rows(cuda_device, c):
+    """Rows 2^31 elements and more from the first one give what they give near by, in place too."""
+    from musc_b200 import ops
+    n, size = 6, (1 << 31) + (1 << 30)
+    bufs = [torch.empty(size, dtype=torch.bfloat16, device=cuda_device) for _ in range(2)]
+    stride = (size - c) // n // 8 * 8
+    far = lambda t, i: bufs[i].as_strided(t.shape, (stride, 1)).copy_(t)
+    g = torch.Generator(device=cuda_device).manual_seed(80)
+    x, delta = (torch.randn(n, c, generator=g, device=cuda_device).bfloat16() for _ in range(2))
+    w = 1 + 0.2 * torch.randn(c, generator=g, device=cuda_device)
+    near_x = x.clone()
+    want = ops.add_rmsnorm(near_x, delta, w, out_dtype=torch.bfloat16)
+    far_x = far(x, 0)
+    assert torch.equal(ops.add_rmsnorm(far_x, far(delta, 1), w, out_dtype=torch.bfloat16), want) and torch.equal(far_x, near_x)
+    out = far(torch.zeros_like(x), 1)
+    ops.add_rmsnorm(near_x, None, w, out_dtype=torch.bfloat16, out=out)
+    assert torch.equal(out, ops.add_rmsnorm(near_x, None, w, out_dtype=torch.bfloat16))
+    if c % 64 == 0:
+        f, a = ops.rotary_frequencies([16, 16], device=cuda_device)
+        pos = torch.randint(0, 1000, (n, 2), generator=g, device=cuda_device).to(torch.int32)
+        want, _ = ops.rotary(x, None, pos, f, a, c // 64)
+        far_x = far(x, 0)
+        ops.rotary(far_x, None, pos, f, a, c // 64, out=(far_x, None))
+        assert torch.equal(far_x, want)
