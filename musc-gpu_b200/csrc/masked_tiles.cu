@@ -17,8 +17,8 @@
 // of both halves take 1024 cycles (16 a cycle and SM), the products 700 for D = 64 and 1350 for D = 128
 // (S of 128 x 64 runs at two thirds of the rate of 128 x 128, whose S would leave no tensor memory
 // for P beside it).  Measured at 8192 tokens of 16 heads, no mask, bf16, calls apart: D = 128 509 us (1080 TF/s,
-// 0.64 of the measured 1693), D = 64 486 us (566 TF/s); four waves of CTAs for 3.46 waves of work.  (18 calls back to
-// back run at lower clocks: D = 128 556 us, D = 64 481.)  The
+// 0.64 of the measured 1693), D = 64 486 us (566 TF/s); four waves of CTAs for 3.46 waves of work.  (In a graph of
+// 18 calls back to back: D = 128 556 us, D = 64 481.)  The
 // special-function unit is 60 % busy, the tensor pipe 29 % (D = 64, ncu): the rest is the softmax warps'
 // own chain, two of them a scheduler.  Tried and dropped, with times at D = 64 or 128: tiles of 128 keys with P over
 // S (548 us), a maximum of every tile before its exponentials (no gain from leaving it out by itself, but
